@@ -10,9 +10,9 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libdiffulex_amd.so"
 
-DFX_ABI_VERSION = 8
+DFX_ABI_VERSION = 9
 DFX_OK = 0
-DFX_KV_BF16, DFX_KV_FP8_E4M3 = 0, 1
+DFX_KV_BF16, DFX_KV_FP8_E4M3, DFX_KV_MX_E4M3, DFX_KV_MX_E2M1 = 0, 1, 2, 3
 DFX_MASK_FULL, DFX_MASK_BLOCK_CAUSAL = 0, 1
 DFX_INDEX_I32, DFX_INDEX_I64 = 0, 1
 DFX_ATTN_GENERIC_PATH = 1
@@ -27,7 +27,7 @@ DFX_WORKSPACE_COUNTER_BYTES = 1 << 18
 EXPORTS = (
     "dfx_abi_version", "dfx_status_string", "dfx_kv_store_unified", "dfx_kv_store_distinct",
     "dfx_kv_load", "dfx_paged_attn_workspace_bytes", "dfx_paged_attn", "dfx_paged_attn_static", "dfx_paged_attn_plan_bytes", "dfx_paged_attn_plan", "dfx_stream_capture_id",
-    "dfx_rope_kv_store", "dfx_build_decode_metadata",
+    "dfx_rope_kv_store", "dfx_build_decode_metadata", "dfx_kv_store_mx", "dfx_kv_load_mx",
 )
 
 
@@ -72,6 +72,7 @@ class RopeParams(C.Structure):
         ("slot_mapping", C.c_void_p), ("slot_index_type", C.c_int32), ("n_slots", C.c_int64),
         ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("cache_layout", C.c_int32), ("page_size", C.c_int32), ("kc_stride", C.c_int64 * 3), ("vc_stride", C.c_int64 * 3),
+        ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("k_block_scales", C.c_void_p), ("v_block_scales", C.c_void_p),
     ]
 
 
@@ -136,6 +137,11 @@ def load() -> C.CDLL:
     lib.dfx_paged_attn_plan.argtypes = [C.POINTER(AttnParams), vp, i64, vp]
     lib.dfx_paged_attn_static.restype = i32
     lib.dfx_paged_attn_static.argtypes = [C.POINTER(AttnParams), vp]
+    lib.dfx_kv_store_mx.restype = i32
+    lib.dfx_kv_store_mx.argtypes = [vp, vp, i64, i64, vp, vp, vp, vp, vp, i32, i64, i64, i32, i32, i32, vp]
+    lib.dfx_kv_load_mx.restype = i32
+    lib.dfx_kv_load_mx.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i64,
+                                   i32, i32, i32, i64, i32, vp]
     lib.dfx_rope_kv_store.restype = i32
     lib.dfx_rope_kv_store.argtypes = [C.POINTER(RopeParams), vp]
     lib.dfx_build_decode_metadata.restype = i32

@@ -11,6 +11,7 @@
 #include "dfx_common.h"
 #include "fp8_e4m3.h"
 #include "distinct_tile.h"
+#include "mx_format.h"
 
 namespace dfx {
 namespace {
@@ -37,6 +38,14 @@ struct RopeArgs {
     // distinct layout (bf16): K [pages, h_kv, hd / 8, page, 8], V [pages, h_kv, hd, page], strides in elements
     int distinct, page_size;
     int64_t kd[3], vd[3];
+    // the general kernel
+    int rot;                        // rotated elements of a head row, the first ones
+    uint8_t* k_scales;              // microscaled caches: scale bytes [n_slots, h_kv, hd / 32]
+    uint8_t* v_scales;
+    const void* positions;
+    const void* slots;
+    int pos_type, slot_type;
+    int items, tokens_per_block;    // work items of a token; tokens of a workgroup
 };
 
 DFX_D u32x4 pack8(const float (&y)[8]) {
@@ -237,6 +246,161 @@ int launch_rope_distinct(const RopeArgs& a, const void* positions, const void* s
     return launch_status();
 }
 
+// ---- the other forms ---------------------------------------------------------------------------
+// Pairs of neighbouring elements (INTERLEAVED: x[2i], x[2i+1] turn by angle i) or of the two halves of the first
+// `rot` elements (x[i], x[i + rot/2]); elements from rot on are copied; stores into microscaled caches.
+//
+// A work item is 16 elements of a head row and 32 bytes of it: both chunks of a pair of halves, 16 neighbouring elements
+// otherwise, so that whoever reads an element is the one who writes it (in place is safe).  The rows are moved once
+// and the angles come from L1 (every head of a token reads the same table row), so memory bounds it.  kUnroll items per
+// thread are loaded before the first is used: one item's loads in flight per thread left the launch waiting on latency.
+constexpr int kUnroll = 4;
+constexpr int kStoreNone = 0, kStoreBf16 = 1, kStoreFp8 = 2, kStoreMx8 = 3, kStoreMx4 = 4;
+
+DFX_D int64_t index_at(const void* p, int64_t i, int type) {
+    return type == DFX_INDEX_I64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// 8 elements [lo, lo + 8) and 8 elements [hi, hi + 8) of one K or V head row into its cache row.  Microscaled: lanes c, c ^ 1, ..
+// of a block hold its chunks -- in the halves layout four lanes hold block lo / 32 and another block hi / 32, otherwise
+// two lanes hold one block between them.
+template <int STORE>
+DFX_D void put_cache(const RopeArgs& a, void* cache, uint8_t* scales, const float* head_scale, int64_t slot, int h, int lo, int hi,
+                     bool halves, u32x4 w1, u32x4 w2) {
+    const int64_t row = (slot * a.h_kv + h) * a.hd;
+    if constexpr (STORE == kStoreBf16) {
+        uint16_t* p = static_cast<uint16_t*>(cache) + row;
+        *reinterpret_cast<u32x4*>(p + lo) = w1;
+        *reinterpret_cast<u32x4*>(p + hi) = w2;
+    } else if constexpr (STORE == kStoreFp8) {
+        uint8_t* p = static_cast<uint8_t*>(cache) + row;
+        *reinterpret_cast<u32x2*>(p + lo) = quantise8(w1, head_scale[h]);
+        *reinterpret_cast<u32x2*>(p + hi) = quantise8(w2, head_scale[h]);
+    } else {
+        constexpr bool E2M1 = STORE == kStoreMx4;
+        uint32_t a1 = abs_max8(w1), a2 = abs_max8(w2);
+        const uint32_t q1 = max_quad(a1), q2 = max_quad(a2), p12 = max_pair(max(a1, a2));
+        a1 = halves ? q1 : p12;
+        a2 = halves ? q2 : p12;
+        uint8_t* codes = static_cast<uint8_t*>(cache) + row / (E2M1 ? 2 : 1);
+        uint8_t* sc = scales + row / kMxBlock;
+        mx_put8<E2M1>(w1, a1, codes, sc, lo >> 3, (lo & 31) == 0);
+        mx_put8<E2M1>(w2, a2, codes, sc, hi >> 3, (hi & 31) == 0);
+    }
+}
+
+template <int STORE, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rope_forms_kernel(const RopeArgs a) {
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
+    const int n = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_block), a.n_tokens - t0)) * a.items;
+    const int cph = a.hd >> 4, turned = a.rot >> 4;
+    for (int base = 0; base < n; base += kThreads * kUnroll) {
+        const uint16_t* src[kUnroll];
+        uint16_t* dst[kUnroll];
+        int lo[kUnroll], hi[kUnroll], head[kUnroll];
+        int64_t tok[kUnroll], pos[kUnroll];
+        u32x4 w1[kUnroll], w2[kUnroll];
+        bool live[kUnroll], turn[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = base + u * kThreads + static_cast<int>(threadIdx.x);
+            live[u] = i < n;
+            const int tt = live[u] ? i / a.items : 0;
+            const int r = live[u] ? i - tt * a.items : 0;
+            head[u] = r / cph;  // q heads, then k heads, then v heads
+            const int c = r - head[u] * cph;
+            tok[u] = t0 + tt;
+            const bool is_v = head[u] >= a.h_q + a.h_kv, is_k = head[u] >= a.h_q && !is_v;
+            const int h = head[u] - (is_v ? a.h_q + a.h_kv : is_k ? a.h_q : 0);
+            // (V rows are copied: two chunks of the row's halves or 16 neighbours, as its K row is)
+            turn[u] = c < turned && !is_v;
+            const bool pair = !INTERLEAVED && c < turned;
+            lo[u] = pair ? c * 8 : c * 16;
+            hi[u] = pair ? lo[u] + (a.rot >> 1) : lo[u] + 8;
+            src[u] = (is_v ? a.v + tok[u] * a.v_st : is_k ? a.k + tok[u] * a.k_st : a.q + tok[u] * a.q_st) + h * a.hd;
+            dst[u] = is_v ? nullptr : (is_k ? a.k_out + tok[u] * a.ko_st : a.q_out + tok[u] * a.qo_st) + h * a.hd;
+            w1[u] = w2[u] = u32x4{0, 0, 0, 0};
+            pos[u] = 0;
+            if (live[u]) {
+                w1[u] = *reinterpret_cast<const u32x4*>(src[u] + lo[u]);
+                w2[u] = *reinterpret_cast<const u32x4*>(src[u] + hi[u]);
+                const int64_t p = index_at(a.positions, tok[u], a.pos_type);
+                pos[u] = p < 0 ? 0 : (p >= a.max_position ? a.max_position - 1 : p);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (!live[u]) continue;
+            if (turn[u]) {
+                // angle indices of the item: 8 of them from the pair index on
+                const int first = INTERLEAVED ? lo[u] >> 1 : lo[u];
+                const float* row = a.table + pos[u] * a.rot + first;
+                float cs[8], sn[8], x1[8], x2[8], y1[8], y2[8];
+                *reinterpret_cast<f32x4*>(cs) = *reinterpret_cast<const f32x4*>(row);
+                *reinterpret_cast<f32x4*>(cs + 4) = *reinterpret_cast<const f32x4*>(row + 4);
+                *reinterpret_cast<f32x4*>(sn) = *reinterpret_cast<const f32x4*>(row + (a.rot >> 1));
+                *reinterpret_cast<f32x4*>(sn + 4) = *reinterpret_cast<const f32x4*>(row + (a.rot >> 1) + 4);
+                if constexpr (INTERLEAVED) {
+                    float e[8], f[8];
+                    unpack8(w1[u], e);
+                    unpack8(w2[u], f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x1[i] = e[2 * i];
+                        x2[i] = e[2 * i + 1];
+                        x1[4 + i] = f[2 * i];
+                        x2[4 + i] = f[2 * i + 1];
+                    }
+                    rotate8(x1, x2, cs, sn, y1, y2);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[2 * i] = y1[i];
+                        e[2 * i + 1] = y2[i];
+                        f[2 * i] = y1[4 + i];
+                        f[2 * i + 1] = y2[4 + i];
+                    }
+                    w1[u] = pack8(e);
+                    w2[u] = pack8(f);
+                } else {
+                    unpack8(w1[u], x1);
+                    unpack8(w2[u], x2);
+                    rotate8(x1, x2, cs, sn, y1, y2);
+                    w1[u] = pack8(y1);
+                    w2[u] = pack8(y2);
+                }
+            }
+            if (dst[u] != nullptr) {
+                *reinterpret_cast<u32x4*>(dst[u] + lo[u]) = w1[u];
+                *reinterpret_cast<u32x4*>(dst[u] + hi[u]) = w2[u];
+            }
+            if constexpr (STORE != kStoreNone) {
+                if (head[u] < a.h_q) continue;
+                const int64_t slot = index_at(a.slots, tok[u], a.slot_type);
+                if (slot < 0 || slot >= a.n_slots) continue;
+                const bool is_v = head[u] >= a.h_q + a.h_kv;
+                const int h = head[u] - a.h_q - (is_v ? a.h_kv : 0);
+                put_cache<STORE>(a, is_v ? a.v_cache : a.k_cache, is_v ? a.v_scales : a.k_scales, is_v ? a.v_scale : a.k_scale, slot, h,
+                                 lo[u], hi[u], hi[u] - lo[u] != 8, w1[u], w2[u]);
+            }
+        }
+    }
+}
+
+template <int STORE>
+int launch_rope_forms(RopeArgs& a, bool interleaved, hipStream_t st) {
+    a.items = (a.h_q + a.h_kv + a.v_heads) * (a.hd >> 4);
+    // (one round of kUnroll items per thread, or one token; fewer tokens per workgroup while that leaves compute units idle)
+    int64_t tokens = kThreads * kUnroll / a.items;
+    if (tokens > a.n_tokens / 512) tokens = a.n_tokens / 512;
+    a.tokens_per_block = tokens < 1 ? 1 : static_cast<int>(tokens);
+    const int64_t blocks = (a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+    if (blocks > UINT32_MAX / kThreads) return DFX_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
+    if (interleaved) hipLaunchKernelGGL((rope_forms_kernel<STORE, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rope_forms_kernel<STORE, false>), grid, block, 0, st, a);
+    return launch_status();
+}
+
 template <bool FP8, typename PosT>
 int launch_rope(const RopeArgs& a, const void* positions, const void* slots, int slot_type, hipStream_t st) {
     const int64_t work = a.n_tokens * (a.h_q + a.h_kv + a.v_heads) * (a.hd >> 4);
@@ -267,7 +431,12 @@ extern "C" int dfx_rope_kv_store(const dfx_rope_params* p, dfx_stream_t stream) 
     if (p->position_index_type != DFX_INDEX_I32 && p->position_index_type != DFX_INDEX_I64) return DFX_ERR_INVALID_ARG;
     const bool store = p->slot_mapping != nullptr;
     const bool fp8 = p->kv_dtype == DFX_KV_FP8_E4M3;
-    if (!fp8 && p->kv_dtype != DFX_KV_BF16) return DFX_ERR_INVALID_ARG;
+    const bool mx = p->kv_dtype == DFX_KV_MX_E4M3 || p->kv_dtype == DFX_KV_MX_E2M1;
+    if (!fp8 && !mx && p->kv_dtype != DFX_KV_BF16) return DFX_ERR_INVALID_ARG;
+    if (p->rotary_dim < 0 || p->rotary_dim > p->head_dim || (p->interleaved != 0 && p->interleaved != 1)) return DFX_ERR_INVALID_ARG;
+    const int rot = p->rotary_dim ? p->rotary_dim : p->head_dim;
+    if (rot % 16 != 0) return DFX_ERR_UNSUPPORTED;
+    const bool forms = rot != p->head_dim || p->interleaved || (store && mx);  // the general kernel
 
     RopeArgs a{};
     a.q = static_cast<const uint16_t*>(p->q);
@@ -302,9 +471,12 @@ extern "C" int dfx_rope_kv_store(const dfx_rope_params* p, dfx_stream_t stream) 
         if (!aligned16(p->k_cache) || !aligned16(p->v_cache)) return DFX_ERR_INVALID_ARG;
         if (p->slot_index_type != DFX_INDEX_I32 && p->slot_index_type != DFX_INDEX_I64) return DFX_ERR_INVALID_ARG;
         if (fp8 != (p->k_scale != nullptr) || fp8 != (p->v_scale != nullptr)) return DFX_ERR_INVALID_ARG;
+        if (mx != (p->k_block_scales != nullptr) || mx != (p->v_block_scales != nullptr)) return DFX_ERR_INVALID_ARG;
         if (p->cache_layout != DFX_CACHE_UNIFIED && p->cache_layout != DFX_CACHE_DISTINCT) return DFX_ERR_INVALID_ARG;
+        // (the chunks of a 32-element block are held by lanes of one quad: heads of whole quads, halves of whole blocks)
+        if (mx && (p->head_dim % 64 != 0 || rot % (p->interleaved ? 32 : 64) != 0)) return DFX_ERR_UNSUPPORTED;
         if (p->cache_layout == DFX_CACHE_DISTINCT) {
-            if (fp8 || (p->head_dim != 64 && p->head_dim != 128)) return DFX_ERR_UNSUPPORTED;
+            if (fp8 || mx || forms || (p->head_dim != 64 && p->head_dim != 128)) return DFX_ERR_UNSUPPORTED;
             if (p->page_size <= 0 || p->n_slots % p->page_size != 0) return DFX_ERR_INVALID_ARG;
             for (int i = 0; i < 3; ++i) {
                 if (p->kc_stride[i] < 0 || p->kc_stride[i] % 8 || p->vc_stride[i] < 0) return DFX_ERR_INVALID_ARG;
@@ -320,10 +492,24 @@ extern "C" int dfx_rope_kv_store(const dfx_rope_params* p, dfx_stream_t stream) 
         a.n_slots = p->n_slots;
         a.k_scale = p->k_scale;
         a.v_scale = p->v_scale;
-    } else if (p->k_cache || p->v_cache || p->k_scale || p->v_scale) {
+    } else if (p->k_cache || p->v_cache || p->k_scale || p->v_scale || p->k_block_scales || p->v_block_scales) {
         return DFX_ERR_INVALID_ARG;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (forms) {
+        a.rot = rot;
+        a.k_scales = static_cast<uint8_t*>(p->k_block_scales);
+        a.v_scales = static_cast<uint8_t*>(p->v_block_scales);
+        a.positions = p->positions;
+        a.slots = p->slot_mapping;
+        a.pos_type = p->position_index_type;
+        a.slot_type = p->slot_index_type;
+        if (static_cast<int64_t>(a.h_q + a.h_kv + a.v_heads) * (a.hd >> 4) > INT32_MAX / 4096) return DFX_ERR_UNSUPPORTED;
+        if (!store) return launch_rope_forms<kStoreNone>(a, p->interleaved, st);
+        if (p->kv_dtype == DFX_KV_MX_E4M3) return launch_rope_forms<kStoreMx8>(a, p->interleaved, st);
+        if (p->kv_dtype == DFX_KV_MX_E2M1) return launch_rope_forms<kStoreMx4>(a, p->interleaved, st);
+        return fp8 ? launch_rope_forms<kStoreFp8>(a, p->interleaved, st) : launch_rope_forms<kStoreBf16>(a, p->interleaved, st);
+    }
     if (a.distinct)
         return p->position_index_type == DFX_INDEX_I64
                    ? launch_rope_distinct<int64_t>(a, p->positions, p->slot_mapping, p->slot_index_type, st)

@@ -5,6 +5,7 @@
 // the exported C function of libdiffulex_amd.so on PyTorch's current HIP stream.  Nothing is
 // computed here and nothing is allocated: outputs and scratch are arguments.  Host code only.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -322,6 +323,83 @@ void kv_load(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_new, 
           "dfx_kv_load");
 }
 
+// ---- microscaled KV cache -----------------------------------------------------------------------
+// E8M0 scale bytes of a cache's 32-element blocks: [pages, page, H_kv, hd / 32].
+bool is_block_scale(const OptTensor& s) { return has(s) && s->dim() == 4 && s->element_size() == 1; }
+
+// The format of a pair of microscaled caches (a head row's bytes say which: hd or hd / 2), all four tensors checked.
+int mx_format(const Tensor& k_cache, const Tensor& v_cache, const Tensor& ks, const Tensor& vs, int64_t heads, int64_t hd) {
+    TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.element_size() == 1 &&
+                    v_cache.element_size() == 1 && k_cache.is_contiguous() && v_cache.is_contiguous() && k_cache.size(2) == heads &&
+                    (k_cache.size(3) == hd || 2 * k_cache.size(3) == hd),
+                "microscaled caches: contiguous one-byte [pages, page, H_kv, hd] (E4M3) or [pages, page, H_kv, hd / 2] (E2M1)");
+    for (const Tensor* s : {&ks, &vs})
+        TORCH_CHECK(s->dim() == 4 && s->element_size() == 1 && s->is_contiguous() && s->size(0) == k_cache.size(0) &&
+                        s->size(1) == k_cache.size(1) && s->size(2) == heads && s->size(3) * 32 == hd,
+                    "block scales: contiguous one-byte (E8M0) [pages, page, H_kv, hd / 32]");
+    for (const Tensor* t : {&k_cache, &v_cache, &ks, &vs}) TORCH_CHECK(t->is_cuda() && t->device() == k_cache.device(), "caches and scales on one device");
+    return k_cache.size(3) == hd ? DFX_KV_MX_E4M3 : DFX_KV_MX_E2M1;
+}
+
+void kv_store_mx(const Tensor& key, const Tensor& value, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale,
+                 const Tensor& slot_mapping) {
+    const c10::DeviceGuard guard(key.device());
+    TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes(), "key, value: [N, H_kv, hd]");
+    const int64_t n = key.size(0), heads = key.size(1), hd = key.size(2);
+    TORCH_CHECK(key.scalar_type() == at::kBFloat16 && value.scalar_type() == at::kBFloat16, "key and value: bf16");
+    TORCH_CHECK(key.stride(2) == 1 && value.stride(2) == 1 && key.stride(1) == hd && value.stride(1) == hd,
+                "key and value rows must be dense");
+    TORCH_CHECK(n == slot_mapping.numel(), "`N`: ", n, ", `slot_mapping.numel()`: ", slot_mapping.numel());
+    TORCH_CHECK(slot_mapping.is_contiguous(), "slot_mapping must be contiguous");
+    const int fmt = mx_format(k_cache, v_cache, k_scale, v_scale, heads, hd);
+    for (const Tensor* t : {&value, static_cast<const Tensor*>(&k_cache), &slot_mapping})
+        TORCH_CHECK(t->device() == key.device(), "all tensors on one device");
+    check(dfx_kv_store_mx(key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+                          k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(),
+                          index_type(slot_mapping, "slot_mapping"), n, k_cache.size(0) * k_cache.size(1), static_cast<int>(heads),
+                          static_cast<int>(hd), fmt, current_stream()),
+          "dfx_kv_store_mx");
+}
+
+void kv_load_mx(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, const Tensor& k_new,
+                const Tensor& v_new, Tensor k_out, Tensor v_out, const Tensor& block_tables, const Tensor& context_lens,
+                const Tensor& seq_lens_new, const Tensor& cu_q, const Tensor& cu_k, int64_t max_total_len) {
+    const c10::DeviceGuard guard(k_cache.device());
+    TORCH_CHECK(k_new.dim() == 3 && k_new.sizes() == v_new.sizes() && k_new.scalar_type() == at::kBFloat16 &&
+                    v_new.scalar_type() == at::kBFloat16,
+                "k_new, v_new: bf16 [N, H_kv, hd]");
+    const int64_t heads = k_new.size(1), hd = k_new.size(2), num_seqs = block_tables.size(0);
+    const int fmt = mx_format(k_cache, v_cache, k_scale, v_scale, heads, hd);
+    TORCH_CHECK(k_new.stride(2) == 1 && k_new.stride(1) == hd && v_new.stride(2) == 1 && v_new.stride(1) == hd,
+                "fresh rows must be dense");
+    check_i32(context_lens, "context_lens");
+    check_i32(seq_lens_new, "seq_lens");
+    check_i32(cu_q, "cu_seqlens_q");
+    check_i32(cu_k, "cu_seqlens_k");
+    TORCH_CHECK(cu_q.numel() == num_seqs + 1 && cu_k.numel() == num_seqs + 1 && context_lens.numel() == num_seqs &&
+                    seq_lens_new.numel() == num_seqs,
+                "context_lens and seq_lens have num_seqs entries, cu_seqlens one more");
+    TORCH_CHECK(block_tables.is_cuda() && block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
+                    (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
+                "block_tables: int32 with dense rows");
+    TORCH_CHECK(k_out.dim() == 3 && k_out.is_contiguous() && v_out.is_contiguous() && k_out.scalar_type() == at::kBFloat16 &&
+                    v_out.scalar_type() == at::kBFloat16 && v_out.sizes() == k_out.sizes() && k_out.size(1) == heads &&
+                    k_out.size(2) == hd,
+                "outputs: contiguous bf16 [total, H_kv, hd]");
+    for (const Tensor* t : {&k_new, &v_new, static_cast<const Tensor*>(&k_out), static_cast<const Tensor*>(&v_out), &block_tables,
+                            &context_lens, &seq_lens_new, &cu_q, &cu_k})
+        TORCH_CHECK(t->device() == k_cache.device(), "all tensors on one device");
+    check(dfx_kv_load_mx(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_new.data_ptr(),
+                         v_new.data_ptr(), k_new.stride(0), v_new.stride(0), k_new.size(0), k_out.data_ptr(), v_out.data_ptr(),
+                         k_out.size(0), static_cast<const int32_t*>(block_tables.data_ptr()), block_tables.stride(0),
+                         static_cast<const int32_t*>(context_lens.data_ptr()),
+                         static_cast<const int32_t*>(seq_lens_new.data_ptr()), static_cast<const int32_t*>(cu_q.data_ptr()),
+                         static_cast<const int32_t*>(cu_k.data_ptr()), static_cast<int>(num_seqs),
+                         static_cast<int>(block_tables.size(1)), k_cache.size(0), static_cast<int>(k_cache.size(1)),
+                         static_cast<int>(heads), static_cast<int>(hd), max_total_len, fmt, current_stream()),
+          "dfx_kv_load_mx");
+}
+
 // ---- rotary embedding (+ KV-cache store) ------------------------------------------------------
 int64_t rows_of(const Tensor& x, int64_t head_size, int64_t& heads, const char* name) {
     TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && (x.dim() == 2 || x.dim() == 3) && x.stride(-1) == 1, name,
@@ -339,7 +417,10 @@ int64_t rows_of(const Tensor& x, int64_t head_size, int64_t& heads, const char* 
 void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& key, Tensor q_out, Tensor k_out,
                    const Tensor& cos_sin_cache, int64_t head_size, const OptTensor& value, const OptTensor& k_cache,
                    const OptTensor& v_cache, const OptTensor& slot_mapping, const OptTensor& k_scale,
-                   const OptTensor& v_scale) {
+                   const OptTensor& v_scale, int64_t rotary_dim, bool interleaved) {
+    const c10::DeviceGuard guard(query.device());
+    TORCH_CHECK(cos_sin_cache.dim() >= 1 && cos_sin_cache.numel() == cos_sin_cache.size(0) * (rotary_dim ? rotary_dim : head_size),
+                "cos_sin_cache: [max_position, rotary_dim]");
     TORCH_CHECK(cos_sin_cache.is_cuda() && cos_sin_cache.scalar_type() == at::kFloat && cos_sin_cache.is_contiguous(),
                 "cos_sin_cache: contiguous fp32 device tensor");
     int64_t hq, hk;
@@ -362,6 +443,8 @@ void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& k
     p.num_q_heads = static_cast<int32_t>(hq);
     p.num_kv_heads = static_cast<int32_t>(hk);
     p.head_dim = static_cast<int32_t>(head_size);
+    p.rotary_dim = static_cast<int32_t>(rotary_dim);
+    p.interleaved = interleaved ? 1 : 0;
     p.kv_dtype = DFX_KV_BF16;
     if (has(slot_mapping)) {
         TORCH_CHECK(has(value) && has(k_cache) && has(v_cache), "the store needs value and both caches");
@@ -383,6 +466,11 @@ void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& k
                 p.kc_stride[i] = k_cache->stride(i);
                 p.vc_stride[i] = v_cache->stride(i);
             }
+        } else if (is_block_scale(k_scale)) {
+            TORCH_CHECK(has(v_scale), "an MX KV cache needs v_scale");
+            p.kv_dtype = mx_format(*k_cache, *v_cache, *k_scale, *v_scale, hk, head_size);
+            p.k_block_scales = k_scale->data_ptr();
+            p.v_block_scales = v_scale->data_ptr();
         } else {
             TORCH_CHECK(k_cache->is_contiguous() && v_cache->is_contiguous() && k_cache->dim() == 4 &&
                             k_cache->stride(1) == row && v_cache->stride(1) == row,
@@ -397,7 +485,7 @@ void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& k
         p.slot_mapping = slot_mapping->data_ptr();
         p.slot_index_type = index_type(*slot_mapping, "slot_mapping");
         p.n_slots = distinct ? k_cache->size(0) * k_cache->size(3) : k_cache->size(0) * k_cache->size(1);
-        if (!distinct && is_fp8_cache(*k_cache)) {
+        if (!distinct && !p.k_block_scales && is_fp8_cache(*k_cache)) {
             p.kv_dtype = DFX_KV_FP8_E4M3;
             p.k_scale = scale_ptr(k_scale, static_cast<int>(hk), "k_scale");
             p.v_scale = scale_ptr(v_scale, static_cast<int>(hk), "v_scale");
@@ -490,8 +578,13 @@ TORCH_LIBRARY(diffulex_amd, m) {
           "Tensor block_tables, Tensor context_lens, Tensor seq_lens_new, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
           "int max_total_len, Tensor? k_scale, Tensor? v_scale) -> ()");
     m.def("rope_kv_store(Tensor positions, Tensor query, Tensor key, Tensor(a!) q_out, Tensor(b!) k_out, Tensor cos_sin_cache, "
-          "int head_size, Tensor? value, Tensor(c!)? k_cache, Tensor(d!)? v_cache, Tensor? slot_mapping, Tensor? k_scale, "
-          "Tensor? v_scale) -> ()");
+          "int head_size, Tensor? value, Tensor(c!)? k_cache, Tensor(d!)? v_cache, Tensor? slot_mapping, Tensor(e!)? k_scale, "
+          "Tensor(f!)? v_scale, int rotary_dim=0, bool interleaved=False) -> ()");
+    m.def("kv_store_mx(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+          "Tensor slot_mapping) -> ()");
+    m.def("kv_load_mx(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor k_new, Tensor v_new, "
+          "Tensor(a!) k_out, Tensor(b!) v_out, Tensor block_tables, Tensor context_lens, Tensor seq_lens_new, "
+          "Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_total_len) -> ()");
     m.def("build_decode_metadata(int strategy, Tensor block_tables, Tensor block_state, int page_size, "
           "int diffusion_block_size, Tensor? num_tokens, Tensor? num_pages, Tensor? prompt_len, "
           "Tensor? num_diffusion_blocks, Tensor(a!) positions, Tensor(b!) slot_mapping, Tensor(c!) cu_seqlens_q, "
@@ -509,5 +602,7 @@ TORCH_LIBRARY_IMPL(diffulex_amd, CUDA, m) {
     m.impl("kv_store_distinct", kv_store_distinct);
     m.impl("kv_load", kv_load);
     m.impl("rope_kv_store", rope_kv_store);
+    m.impl("kv_store_mx", kv_store_mx);
+    m.impl("kv_load_mx", kv_load_mx);
     m.impl("build_decode_metadata", build_decode_metadata);
 }

@@ -5,6 +5,12 @@ An FP8 cache is recognised by its dtype (``torch.float8_e4m3fn``, or ``uint8``
 holding the codes); its per-KV-head scales come from the ``k_scale`` /
 ``v_scale`` keyword arguments or, if absent, from attributes of the same names
 on ``attn_metadata``.
+
+A microscaled (MX) cache is recognised by its scales: ``k_scale`` / ``v_scale`` of shape
+``[pages, page, H_kv, hd / 32]`` and one-byte elements (``torch.float8_e8m0fnu`` or ``uint8``), one power of two per
+32 elements of a head row, written by the store along with the codes.  The codes are E4M3
+(``[pages, page, H_kv, hd]``) or E2M1 (``[pages, page, H_kv, hd / 2]``, two to a byte), as the cache's last
+dimension says.
 """
 from __future__ import annotations
 
@@ -27,6 +33,10 @@ def _index_type(t: torch.Tensor) -> int:
     if t.dtype == torch.int64:
         return _lib.DFX_INDEX_I64
     raise AssertionError(f"slot_mapping must be int32 or int64, got {t.dtype}")
+
+
+def _is_block_scale(scale) -> bool:
+    return scale is not None and scale.dim() == 4 and scale.element_size() == 1
 
 
 def _scales(cache: torch.Tensor, attn_metadata, k_scale, v_scale, n_heads: int):
@@ -58,7 +68,13 @@ def store_kvcache_unified_layout(key: torch.Tensor, value: torch.Tensor,
                                  slot_mapping: torch.Tensor, attn_metadata,
                                  k_scale: Optional[torch.Tensor] = None,
                                  v_scale: Optional[torch.Tensor] = None) -> None:
-    """kv_cache_kernels.py:110-124.  key/value: [N, H_kv, hd]; caches: [pages, page, H_kv, hd]."""
+    """kv_cache_kernels.py:110-124.  key/value: [N, H_kv, hd]; caches: [pages, page, H_kv, hd].
+    Block scales (module docstring): the rows are quantised block by block and their scales written as well."""
+    if _is_block_scale(k_scale):
+        slots = slot_mapping.reshape(-1)
+        _call(_lib.ops().kv_store_mx, key, value, k_cache, v_cache, k_scale, v_scale,
+              slots if slots.is_contiguous() else slots.contiguous())
+        return
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     assert key.stride(-1) == 1 and value.stride(-1) == 1
@@ -98,10 +114,18 @@ def store_kvcache_distinct_layout(key: torch.Tensor, value: torch.Tensor,
 def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, attn_metadata,
                  k_new: torch.Tensor, v_new: torch.Tensor,
                  k_scale: Optional[torch.Tensor] = None,
-                 v_scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 v_scale: Optional[torch.Tensor] = None,
+                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """kv_cache_kernels.py:230-279.  Returns (k_out, v_out): [sum(ctx + new), H_kv, hd] in
     the cache's dtype.  Unlike the reference kernel a context that fills its last page
-    exactly is copied completely."""
+    exactly is copied completely.
+
+    A microscaled cache (block scales, module docstring) is widened: bf16 outputs, the cached rows as their codes and
+    scales say, the fresh rows as they are.  ``out`` (extension, microscaled caches): the caller's two output
+    tensors, which also spares the host read of their size where ``attn_metadata.max_seqlen_k`` is set."""
+    if _is_block_scale(k_scale):
+        return _load_mx(k_cache, v_cache, attn_metadata, k_new, v_new, k_scale, v_scale, out)
+    assert out is None, "`out` is for microscaled caches"
     assert k_cache.shape == v_cache.shape
     assert k_new.shape == v_new.shape
     N_BLOCKS, PAGE_SIZE, H_KV, HEAD_DIM = k_cache.shape
@@ -133,3 +157,15 @@ def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, attn_metadata,
     _call(_lib.ops().kv_load, k_cache, v_cache, k_new, v_new, k_output, v_output, bt, ctxlens, seqlens,
           cu_seqlens_q, cu_seqlens_k, max_total, ks, vs)
     return k_output, v_output
+
+
+def _load_mx(k_cache, v_cache, md, k_new, v_new, k_scale, v_scale, out):
+    max_total = int(getattr(md, "max_seqlen_k", 0) or 0)
+    if max_total <= 0:
+        max_total = int((md.context_lens + md.seq_lens_ts).max().item()) if md.context_lens.numel() else 0
+    if out is None:
+        total = int(md.cu_seqlens_k[-1].item())  # (one host read, as in load_kvcache)
+        out = tuple(torch.empty((total,) + tuple(k_new.shape[1:]), device=k_cache.device, dtype=torch.bfloat16) for _ in range(2))
+    _call(_lib.ops().kv_load_mx, k_cache, v_cache, k_scale, v_scale, k_new, v_new, out[0], out[1], md.block_tables, md.context_lens,
+          md.seq_lens_ts, md.cu_seqlens_q, md.cu_seqlens_k, max_total)
+    return out[0], out[1]

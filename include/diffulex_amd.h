@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define DFX_ABI_VERSION 8
+#define DFX_ABI_VERSION 9
 
 typedef void* dfx_stream_t; /* a hipStream_t; NULL is the default stream */
 
@@ -34,7 +34,12 @@ typedef enum dfx_status {
 
 typedef enum dfx_kv_dtype {
     DFX_KV_BF16 = 0,    /* 2-byte elements, copied bit for bit (bf16; fp16 works for store/load) */
-    DFX_KV_FP8_E4M3 = 1 /* OCP e4m3fn codes with one fp32 scale per KV head */
+    DFX_KV_FP8_E4M3 = 1, /* OCP e4m3fn codes with one fp32 scale per KV head */
+    /* Microscaled: codes with one power-of-two scale (E8M0 byte b: 2^(b - 127), 255: NaN) per 32 consecutive
+     * elements of a head row, chosen when the row is written; dfx_kv_store_mx, dfx_kv_load_mx, dfx_split_attn,
+     * dfx_rope_kv_store. */
+    DFX_KV_MX_E4M3 = 2, /* e4m3fn codes, head_dim bytes a head row */
+    DFX_KV_MX_E2M1 = 3  /* e2m1 codes, head_dim / 2 bytes a head row, element 2 i in the low half of byte i */
 } dfx_kv_dtype;
 
 typedef enum dfx_mask_mode {
@@ -122,6 +127,33 @@ int dfx_kv_load(const void* k_cache, const void* v_cache, const void* k_new, con
                 int num_seqs, int max_pages_per_seq, int64_t n_pages, int page_size, int n_kv_heads,
                 int head_dim, int64_t max_total_len, int kv_dtype, const float* k_scale,
                 const float* v_scale, dfx_stream_t stream);
+
+/*
+ * Microscaled KV cache: store and load.  No counterpart in the reference.
+ *
+ * k_cache / v_cache: codes [n_slots, n_kv_heads, head_dim or head_dim / 2 bytes] dense (kv_dtype DFX_KV_MX_E4M3 /
+ * DFX_KV_MX_E2M1); k_scales / v_scales: [n_slots, n_kv_heads, head_dim / 32] E8M0 bytes, dense.  For each block
+ * of 32 elements x of a key or value head row with largest magnitude A, the store writes the scale byte b = 127 + e, e
+ * the smallest integer >= -127 with A <= M * 2^e (M = 448 for E4M3, 6 for E2M1), and for each element the code nearest to
+ * x * 2^-e (ties to even).  A block with an infinity or NaN gets b = 255 (it reads back as NaN) and codes 0.
+ * Slots as in dfx_kv_store_unified (slots < 0 or >= n_slots are skipped).
+ *
+ * dfx_kv_load_mx gathers like dfx_kv_load but widens to bf16 (exactly: a code has at most 4 significant bits): rows
+ * [cu_seqlens_k[s], + context_lens[s]) of k_out / v_out ([n_out, n_kv_heads, head_dim] bf16, dense) from the cache, then
+ * seq_lens_new[s] rows of k_new / v_new ([n_new, ..] bf16) as they are.  Rows of skipped pages (table entry < 0 or
+ * >= n_pages) and rows at or beyond n_out are not written; fresh rows at or beyond n_new are not read.
+ *
+ * head_dim a multiple of 32 (DFX_ERR_UNSUPPORTED otherwise); strides (elements) multiples of 8, pointers 16-byte aligned.
+ */
+int dfx_kv_store_mx(const void* key, const void* value, int64_t key_stride, int64_t value_stride, void* k_cache,
+                    void* v_cache, void* k_scales, void* v_scales, const void* slot_mapping, int slot_index_type,
+                    int64_t n_tokens, int64_t n_slots, int n_kv_heads, int head_dim, int kv_dtype, dfx_stream_t stream);
+int dfx_kv_load_mx(const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
+                   const void* k_new, const void* v_new, int64_t k_new_stride, int64_t v_new_stride, int64_t n_new,
+                   void* k_out, void* v_out, int64_t n_out, const int32_t* block_tables, int64_t block_table_stride,
+                   const int32_t* context_lens, const int32_t* seq_lens_new, const int32_t* cu_seqlens_q,
+                   const int32_t* cu_seqlens_k, int num_seqs, int max_pages_per_seq, int64_t n_pages, int page_size,
+                   int n_kv_heads, int head_dim, int64_t max_total_len, int kv_dtype, dfx_stream_t stream);
 
 /*
  * Block-diffusion paged attention.
@@ -429,7 +461,16 @@ int dfx_paged_attn_static(const dfx_attn_params* params, dfx_stream_t stream);
  * or >= n_slots skipped; FP8 caches quantise the bf16-rounded rotated K).
  * slot_mapping == NULL: v, k_cache, v_cache, k_scale, v_scale must be NULL.
  *
- * Supported: head_dim a multiple of 16; heads dense inside a token row; strides
+ * Other forms (no counterpart in the reference, which asserts rotary_dim == head_size):
+ *   rotary_dim: only the first rotary_dim elements of a head are rotated (the halves are those of the first rotary_dim
+ *     elements), the others are copied; the table is then [max_position, rotary_dim].  0 means head_dim.
+ *   interleaved: 1 rotates the pairs (x[2i], x[2i + 1]) by angle i instead of (x[i], x[rotary_dim / 2 + i]).
+ *   Scaled frequencies are a matter of the table's contents alone.
+ *   kv_dtype DFX_KV_MX_*: the store writes a microscaled cache, as dfx_kv_store_mx would write the bf16-rounded rotated K
+ *     and V (k_block_scales / v_block_scales; head_dim a multiple of 64, rotary_dim of 64, or of 32 if interleaved).
+ *   DFX_ERR_UNSUPPORTED: a store into the distinct layout with any of these.
+ *
+ * Supported: head_dim and rotary_dim multiples of 16; heads dense inside a token row; strides
  * (elements) multiples of 8; every pointer 16-byte aligned.
  */
 typedef struct dfx_rope_params {
@@ -463,6 +504,10 @@ typedef struct dfx_rope_params {
     int32_t page_size;
     int64_t kc_stride[3];
     int64_t vc_stride[3];
+    int32_t rotary_dim;  /* 0: head_dim */
+    int32_t interleaved; /* 0: halves, 1: neighbouring elements */
+    void* k_block_scales; /* [n_slots, num_kv_heads, head_dim / 32] E8M0 bytes, DFX_KV_MX_* caches only */
+    void* v_block_scales;
 } dfx_rope_params;
 
 int dfx_rope_kv_store(const dfx_rope_params* params, dfx_stream_t stream);
