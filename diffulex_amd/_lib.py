@@ -28,6 +28,7 @@ EXPORTS = (
     "dfx_abi_version", "dfx_status_string", "dfx_kv_store_unified", "dfx_kv_store_distinct",
     "dfx_kv_load", "dfx_paged_attn_workspace_bytes", "dfx_paged_attn", "dfx_paged_attn_static", "dfx_paged_attn_plan_bytes", "dfx_paged_attn_plan", "dfx_stream_capture_id",
     "dfx_rope_kv_store", "dfx_build_decode_metadata", "dfx_kv_store_mx", "dfx_kv_load_mx",
+    "dfx_split_attn", "dfx_split_attn_workspace_bytes",
 )
 
 
@@ -73,6 +74,29 @@ class RopeParams(C.Structure):
         ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("cache_layout", C.c_int32), ("page_size", C.c_int32), ("kc_stride", C.c_int64 * 3), ("vc_stride", C.c_int64 * 3),
         ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("k_block_scales", C.c_void_p), ("v_block_scales", C.c_void_p),
+    ]
+
+
+class SplitAttnParams(C.Structure):
+    """Mirror of ``dfx_split_attn_params``."""
+    _fields_ = [
+        ("q", C.c_void_p), ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("out", C.c_void_p),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("block_tables", C.c_void_p), ("context_lens", C.c_void_p),
+        ("cu_seqlens_q", C.c_void_p), ("cu_seqlens_new", C.c_void_p),
+        ("prefix_cu_seqs", C.c_void_p), ("prefix_lens", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("q_stride_token", C.c_int64), ("q_stride_head", C.c_int64),
+        ("kn_stride_token", C.c_int64), ("kn_stride_head", C.c_int64),
+        ("vn_stride_token", C.c_int64), ("vn_stride_head", C.c_int64),
+        ("o_stride_token", C.c_int64), ("o_stride_head", C.c_int64),
+        ("cache_stride_page", C.c_int64), ("cache_stride_token", C.c_int64), ("cache_stride_head", C.c_int64),
+        ("block_table_stride", C.c_int64), ("n_pages", C.c_int64),
+        ("num_q_tokens", C.c_int64), ("num_new_tokens", C.c_int64),
+        ("num_seqs", C.c_int32), ("num_groups", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_pages_per_seq", C.c_int32),
+        ("diffusion_block_size", C.c_int32), ("kv_dtype", C.c_int32), ("mask_mode", C.c_int32),
+        ("max_workgroups", C.c_int32), ("scale", C.c_float),
     ]
 
 
@@ -142,6 +166,10 @@ def load() -> C.CDLL:
     lib.dfx_kv_load_mx.restype = i32
     lib.dfx_kv_load_mx.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i64,
                                    i32, i32, i32, i64, i32, vp]
+    lib.dfx_split_attn_workspace_bytes.restype = i64
+    lib.dfx_split_attn_workspace_bytes.argtypes = [C.POINTER(SplitAttnParams)]
+    lib.dfx_split_attn.restype = i32
+    lib.dfx_split_attn.argtypes = [C.POINTER(SplitAttnParams), vp]
     lib.dfx_rope_kv_store.restype = i32
     lib.dfx_rope_kv_store.argtypes = [C.POINTER(RopeParams), vp]
     lib.dfx_build_decode_metadata.restype = i32

@@ -400,6 +400,119 @@ void kv_load_mx(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_sc
           "dfx_kv_load_mx");
 }
 
+// ---- split attention: microscaled caches, shared prefixes ----------------------------------------
+int64_t split_attention_workspace_bytes(const Tensor& q, int64_t num_kv_heads, int64_t num_seqs, int64_t num_groups, int64_t max_wg) {
+    const c10::DeviceGuard guard(q.device());
+    dfx_split_attn_params p = {};
+    p.num_q_tokens = q.size(0);
+    p.num_q_heads = static_cast<int32_t>(q.size(1));
+    p.head_dim = static_cast<int32_t>(q.size(2));
+    p.num_kv_heads = static_cast<int32_t>(num_kv_heads);
+    p.num_seqs = static_cast<int32_t>(num_seqs);
+    p.num_groups = static_cast<int32_t>(num_groups);
+    p.max_workgroups = static_cast<int32_t>(max_wg);
+    const int64_t n = dfx_split_attn_workspace_bytes(&p);
+    if (n < 0) check(static_cast<int>(n), "dfx_split_attn_workspace_bytes");
+    return n;
+}
+
+void split_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& k_cache, const OptTensor& v_cache,
+                     const OptTensor& k_scale, const OptTensor& v_scale, Tensor out, const OptTensor& block_tables,
+                     const OptTensor& context_lens, const Tensor& cu_q, const Tensor& cu_new, const OptTensor& prefix_cu_seqs,
+                     const OptTensor& prefix_lens, Tensor workspace, double scale, int64_t mask_mode, int64_t dbs, int64_t max_wg) {
+    const c10::DeviceGuard guard(q.device());
+    TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16,
+                "q, k and v must be bf16 device tensors");
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes(), "q: [T, H_q, hd]; k, v: [T_new, H_kv, hd]");
+    TORCH_CHECK(q.stride(2) == 1 && k.stride(2) == 1 && v.stride(2) == 1, "the head dimension must be dense");
+    const int64_t h_q = q.size(1), hd = q.size(2), h_kv = k.size(1);
+    TORCH_CHECK(k.size(2) == hd && h_kv > 0 && h_q % h_kv == 0, "head counts / head_dim of q and k do not fit");
+    TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.stride(2) == 1,
+                "out must be a bf16 device tensor shaped like q");
+    check_i32(cu_q, "cu_seqlens_q");
+    check_i32(cu_new, "cu_seqlens_new");
+    const int64_t num_seqs = cu_q.numel() - 1;
+    TORCH_CHECK(num_seqs >= 0 && cu_new.numel() == num_seqs + 1, "cu_seqlens_q and cu_seqlens_new differ in length");
+    auto here = [&](const Tensor& t) { TORCH_CHECK(t.device() == q.device(), "all tensors on one device"); };
+    for (const Tensor* t : {&k, &v, static_cast<const Tensor*>(&out), &cu_q, &cu_new, static_cast<const Tensor*>(&workspace)}) here(*t);
+    dfx_split_attn_params p = {};
+    p.kv_dtype = DFX_KV_BF16;
+    TORCH_CHECK(has(k_cache) == has(v_cache), "k_cache and v_cache come together");
+    if (has(k_cache)) {
+        here(*k_cache);
+        TORCH_CHECK(has(block_tables) && has(context_lens), "a cache needs block_tables and context_lens");
+        here(*block_tables);
+        here(*context_lens);
+        TORCH_CHECK(block_tables->scalar_type() == at::kInt && block_tables->dim() == 2 &&
+                        (block_tables->stride(1) == 1 || block_tables->size(1) <= 1) && block_tables->size(0) == num_seqs,
+                    "block_tables must be int32 [num_seqs, max_pages] with dense rows");
+        check_i32(*context_lens, "context_lens");
+        TORCH_CHECK(context_lens->numel() == num_seqs, "context_lens must have one entry per sequence");
+        if (is_block_scale(k_scale)) {
+            TORCH_CHECK(has(v_scale), "an MX KV cache needs v_scale");
+            p.kv_dtype = mx_format(*k_cache, *v_cache, *k_scale, *v_scale, h_kv, hd);
+            p.k_scales = k_scale->data_ptr();
+            p.v_scales = v_scale->data_ptr();
+        } else {
+            TORCH_CHECK(k_cache->scalar_type() == at::kBFloat16 && v_cache->scalar_type() == at::kBFloat16 && k_cache->dim() == 4 &&
+                            k_cache->sizes() == v_cache->sizes() && k_cache->size(2) == h_kv && k_cache->size(3) == hd &&
+                            k_cache->strides() == v_cache->strides() && k_cache->stride(3) == 1 && v_cache->device() == q.device(),
+                        "shared prefixes: bf16 caches [pages, page, H_kv, hd], laid out alike, or microscaled ones");
+            p.cache_stride_page = k_cache->stride(0);
+            p.cache_stride_token = k_cache->stride(1);
+            p.cache_stride_head = k_cache->stride(2);
+        }
+        p.k_cache = k_cache->data_ptr();
+        p.v_cache = v_cache->data_ptr();
+        p.block_tables = static_cast<const int32_t*>(block_tables->data_ptr());
+        p.context_lens = static_cast<const int32_t*>(context_lens->data_ptr());
+        p.block_table_stride = block_tables->stride(0);
+        p.max_pages_per_seq = static_cast<int32_t>(block_tables->size(1));
+        p.n_pages = k_cache->size(0);
+        p.page_size = static_cast<int32_t>(k_cache->size(1));
+    }
+    TORCH_CHECK(prefix_cu_seqs.has_value() == prefix_lens.has_value(), "prefix_cu_seqs and prefix_lens go together");
+    if (prefix_lens.has_value() && prefix_lens->numel() > 0) {
+        check_i32(*prefix_cu_seqs, "prefix_cu_seqs");
+        check_i32(*prefix_lens, "prefix_lens");
+        here(*prefix_cu_seqs);
+        here(*prefix_lens);
+        TORCH_CHECK(prefix_cu_seqs->numel() == prefix_lens->numel() + 1, "prefix_cu_seqs has one entry more than prefix_lens");
+        TORCH_CHECK(has(k_cache), "a shared prefix lies in a cache");
+        p.prefix_cu_seqs = static_cast<const int32_t*>(prefix_cu_seqs->data_ptr());
+        p.prefix_lens = static_cast<const int32_t*>(prefix_lens->data_ptr());
+        p.num_groups = static_cast<int32_t>(prefix_lens->numel());
+    }
+    p.q = q.data_ptr();
+    p.k_new = k.data_ptr();
+    p.v_new = v.data_ptr();
+    p.out = out.data_ptr();
+    p.cu_seqlens_q = static_cast<const int32_t*>(cu_q.data_ptr());
+    p.cu_seqlens_new = static_cast<const int32_t*>(cu_new.data_ptr());
+    TORCH_CHECK(workspace.is_contiguous(), "workspace must be contiguous");
+    p.workspace = workspace.data_ptr();
+    p.workspace_bytes = workspace.numel() * workspace.element_size();
+    p.q_stride_token = q.stride(0);
+    p.q_stride_head = q.stride(1);
+    p.kn_stride_token = k.stride(0);
+    p.kn_stride_head = k.stride(1);
+    p.vn_stride_token = v.stride(0);
+    p.vn_stride_head = v.stride(1);
+    p.o_stride_token = out.stride(0);
+    p.o_stride_head = out.stride(1);
+    p.num_q_tokens = q.size(0);
+    p.num_new_tokens = k.size(0);
+    p.num_seqs = static_cast<int32_t>(num_seqs);
+    p.num_q_heads = static_cast<int32_t>(h_q);
+    p.num_kv_heads = static_cast<int32_t>(h_kv);
+    p.head_dim = static_cast<int32_t>(hd);
+    p.diffusion_block_size = static_cast<int32_t>(dbs);
+    p.mask_mode = static_cast<int32_t>(mask_mode);
+    p.max_workgroups = static_cast<int32_t>(max_wg);
+    p.scale = static_cast<float>(scale);
+    check(dfx_split_attn(&p, current_stream()), "dfx_split_attn");
+}
+
 // ---- rotary embedding (+ KV-cache store) ------------------------------------------------------
 int64_t rows_of(const Tensor& x, int64_t head_size, int64_t& heads, const char* name) {
     TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && (x.dim() == 2 || x.dim() == 3) && x.stride(-1) == 1, name,
@@ -580,6 +693,11 @@ TORCH_LIBRARY(diffulex_amd, m) {
     m.def("rope_kv_store(Tensor positions, Tensor query, Tensor key, Tensor(a!) q_out, Tensor(b!) k_out, Tensor cos_sin_cache, "
           "int head_size, Tensor? value, Tensor(c!)? k_cache, Tensor(d!)? v_cache, Tensor? slot_mapping, Tensor(e!)? k_scale, "
           "Tensor(f!)? v_scale, int rotary_dim=0, bool interleaved=False) -> ()");
+    m.def("split_attention(Tensor q, Tensor k, Tensor v, Tensor? k_cache, Tensor? v_cache, Tensor? k_scale, Tensor? v_scale, "
+          "Tensor(a!) out, Tensor? block_tables, Tensor? context_lens, Tensor cu_seqlens_q, Tensor cu_seqlens_new, "
+          "Tensor? prefix_cu_seqs, Tensor? prefix_lens, Tensor(b!) workspace, float scale, int mask_mode, int diffusion_block_size, "
+          "int max_workgroups) -> ()");
+    m.def("split_attention_workspace_bytes(Tensor q, int num_kv_heads, int num_seqs, int num_groups, int max_workgroups) -> int");
     m.def("kv_store_mx(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
           "Tensor slot_mapping) -> ()");
     m.def("kv_load_mx(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor k_new, Tensor v_new, "
@@ -603,6 +721,8 @@ TORCH_LIBRARY_IMPL(diffulex_amd, CUDA, m) {
     m.impl("kv_load", kv_load);
     m.impl("rope_kv_store", rope_kv_store);
     m.impl("kv_store_mx", kv_store_mx);
+    m.impl("split_attention", split_attention);
+    m.impl("split_attention_workspace_bytes", split_attention_workspace_bytes);
     m.impl("kv_load_mx", kv_load_mx);
     m.impl("build_decode_metadata", build_decode_metadata);
 }

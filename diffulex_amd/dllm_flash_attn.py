@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .kv_cache_kernels import _FP8_DTYPES, _stream
+from .kv_cache_kernels import _FP8_DTYPES, _call, _is_block_scale, _stream, store_kvcache_unified_layout
 
 class _Workspace:
     __slots__ = ("tensor", "zeroed")
@@ -61,7 +61,8 @@ def paged_attention(q, k, v, k_cache, v_cache, scale, *, block_tables, context_l
                     cu_seqlens_new, max_seqlen_q, mask_mode=_lib.DFX_MASK_FULL, diffusion_block_size=32,
                     k_scale=None, v_scale=None, max_workgroups=0, out=None, flags=0,
                     store_slot_mapping=None, static_scratch=False, plan_cache=None,
-                    cache_layout="unified", rope=None, k_rotated=None) -> torch.Tensor:
+                    cache_layout="unified", rope=None, k_rotated=None, prefix_cu_seqs=None,
+                    prefix_lens=None) -> torch.Tensor:
     """Launch ``dfx_paged_attn`` on the current stream through ``torch.ops.diffulex_amd.paged_attention``
     (which checks the tensors and fills ``dfx_attn_params``).  q: [T, H_q, hd]; k, v: [T_new, H_kv, hd];
     caches [pages, page, H_kv, hd] or None.  ``store_slot_mapping`` ([T_new] int32/int64): the same
@@ -83,7 +84,24 @@ def paged_attention(q, k, v, k_cache, v_cache, scale, *, block_tables, context_l
     launch applies itself (``dfx_attn_params.rope_cos_sin``): query rows on their way into the matrix
     instructions, fresh key rows into ``k_rotated`` (a new [T_new, H_kv, hd] tensor by default) and, with
     ``store_slot_mapping``, into the cache.  Raises ``DfxError`` (unsupported shape) where the pipelined
-    kernels do not run; ``rope_supported()`` tells beforehand."""
+    kernels do not run; ``rope_supported()`` tells beforehand.
+
+    Microscaled caches (``k_scale`` / ``v_scale`` of shape [pages, page, H_kv, hd / 32], one byte each: see
+    ``kv_cache_kernels``) and shared prefixes go through ``dfx_split_attn``, which keeps no plan.
+    ``prefix_cu_seqs`` [G + 1], ``prefix_lens`` [G] (int32 device tensors): the neighbouring sequences
+    ``prefix_cu_seqs[g]`` .. ``prefix_cu_seqs[g + 1]`` hold the same keys at the first ``prefix_lens[g]`` positions of their
+    contexts; they are read once for all of them, through the first one's block-table row (bf16 or microscaled caches in
+    the unified layout).  The fused forms -- ``rope``, ``static_scratch`` -- are not offered there; ``store_slot_mapping`` is,
+    as a launch of its own behind the attention."""
+    if prefix_lens is not None or _is_block_scale(k_scale):
+        if rope is not None or static_scratch or cache_layout != "unified":
+            raise _lib.DfxError("dfx_split_attn: microscaled caches and shared prefixes take the unified layout, without rope and "
+                                "static_scratch (unsupported shape)")
+        out = _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_lens, cu_seqlens_q, cu_seqlens_new,
+                               mask_mode, diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens)
+        if store_slot_mapping is not None:
+            store_kvcache_unified_layout(k, v, k_cache, v_cache, store_slot_mapping, None, k_scale, v_scale)
+        return out
     ops = _lib.ops()
     T, H_q, hd = q.shape
     H_kv = k.shape[1]
@@ -145,6 +163,31 @@ def paged_attention(q, k, v, k_cache, v_cache, scale, *, block_tables, context_l
         if "dfx_" in str(e):
             raise _lib.DfxError(str(e).split("\n")[0]) from None
         raise
+    return out
+
+
+_split_need = {}   # launch shape -> dfx_split_attn_workspace_bytes
+
+
+def _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_lens, cu_seqlens_q, cu_seqlens_new, mask_mode,
+                     diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens):
+    """``dfx_split_attn``.  Its workspace needs no particular contents, so each call takes one from PyTorch's allocator (which
+    orders its reuse on the stream, and gives a captured graph memory of its own)."""
+    ops = _lib.ops()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k_cache is not None and k_cache.numel() == 0:
+        k_cache = v_cache = None
+    num_seqs = cu_seqlens_q.numel() - 1
+    groups = prefix_lens.numel() if prefix_lens is not None else 0
+    key = (q.device.index, q.shape, k.shape[1], num_seqs, groups, max_workgroups)
+    need = _split_need.get(key)
+    if need is None:
+        need = _split_need[key] = int(_call(ops.split_attention_workspace_bytes, q, k.shape[1], num_seqs, groups, int(max_workgroups)))
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _call(ops.split_attention, q, k, v, k_cache, v_cache, k_scale, v_scale, out, block_tables, context_lens, cu_seqlens_q,
+          cu_seqlens_new, prefix_cu_seqs, prefix_lens, workspace, float(scale), int(mask_mode), int(diffusion_block_size),
+          int(max_workgroups))
     return out
 
 
@@ -260,6 +303,8 @@ def dllm_flash_attn_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
     ``scale`` is honoured in both modes.  ``attn_metadata.decode_mask ==
     "block_causal"`` (optional attribute) selects the block-causal mask among the
     in-flight blocks; the default is the reference's behaviour, all fresh tokens visible.
+    ``attn_metadata.prefix_cu_seqs`` / ``prefix_lens`` (optional attributes): groups of sequences that share a prefix;
+    ``k_scale`` / ``v_scale`` with four dimensions: microscaled caches (both: see ``paged_attention``).
     """
     if attn_metadata.decode_mode == "static":
         cu_new = attn_metadata.cu_seqlens_k
@@ -270,6 +315,14 @@ def dllm_flash_attn_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
     mask = _lib.DFX_MASK_FULL
     if getattr(attn_metadata, "decode_mask", "full") == "block_causal":
         mask = _lib.DFX_MASK_BLOCK_CAUSAL
+    prefix_lens = getattr(attn_metadata, "prefix_lens", None)
+    if prefix_lens is not None or _is_block_scale(k_scale):
+        return paged_attention(
+            q, k, v, k_cache, v_cache, scale, block_tables=attn_metadata.block_tables,
+            context_lens=attn_metadata.context_lens, cu_seqlens_q=attn_metadata.cu_seqlens_q, cu_seqlens_new=cu_new,
+            max_seqlen_q=0, mask_mode=mask, diffusion_block_size=attn_metadata.diffusion_block_size, k_scale=k_scale,
+            v_scale=v_scale, store_slot_mapping=store_slot_mapping, cache_layout=kv_cache_layout, rope=rope,
+            prefix_cu_seqs=getattr(attn_metadata, "prefix_cu_seqs", None), prefix_lens=prefix_lens)
     if kv_cache_layout == "distinct":
         return paged_attention(
             q, k, v, k_cache, v_cache, scale, block_tables=attn_metadata.block_tables,

@@ -47,6 +47,10 @@ class PagedAttnMetaData(AttnMetaDataBase):
     k_scale: Optional[torch.Tensor] = None   # fp32 [H_kv], FP8 caches only
     v_scale: Optional[torch.Tensor] = None
     decode_mask: str = "full"                # "full" | "block_causal"
+    # groups of neighbouring sequences that share a prefix (decode; both or neither): sequences prefix_cu_seqs[g] ..
+    # prefix_cu_seqs[g + 1] hold the same keys at the first prefix_lens[g] positions of their contexts
+    prefix_cu_seqs: Optional[torch.Tensor] = None   # int32 [G + 1]
+    prefix_lens: Optional[torch.Tensor] = None      # int32 [G]
 
     def __post_init__(self):
         if self.context_lens is not None:

@@ -512,6 +512,67 @@ typedef struct dfx_rope_params {
 
 int dfx_rope_kv_store(const dfx_rope_params* params, dfx_stream_t stream);
 
+/*
+ * Paged decode attention over microscaled caches, and of groups of sequences that share a prefix.
+ * No counterpart in the reference (whose dllm_flash_attn_decode reads every sequence's prefix for itself).
+ *
+ * The result is that of dfx_paged_attn on the same context_lens, block_tables and fresh rows (masks, skipped pages, rows
+ * without a key: as documented there), for kv_dtype DFX_KV_BF16 and DFX_KV_MX_*; a cache element is its code times its block's
+ * scale, the fresh rows are the bf16 operands.
+ *
+ * Groups (num_groups > 0): sequences prefix_cu_seqs[g] .. prefix_cu_seqs[g + 1) -- neighbours in the batch; sequences before the
+ * first or behind the last group have no shared prefix -- hold the same keys at positions [0, prefix_lens[g]) of
+ * their contexts, which are read ONCE for all of them, through the block table of the group's first sequence; every
+ * sequence's keys from prefix_lens[g] on come through its own table row.  The other sequences' table entries below
+ * prefix_lens[g] / page_size are not read.  A sequence whose context is shorter than its group's prefix sees its context_lens keys
+ * of it.
+ *
+ * Two launches (pieces, merge), planned on the device from the lengths: nothing is read back, both may be recorded into a
+ * graph whose replays find other lengths, and the results do not depend on timing (pieces are merged in order).  The workspace
+ * (dfx_split_attn_workspace_bytes(), 256-byte aligned, any contents) must not be shared by calls that overlap in time.
+ *
+ * Supported: head_dim 64 or 128; num_q_heads a multiple of num_kv_heads; any page_size >= 1; num_seqs <= 65535; strides in
+ * elements, multiples of 8, innermost dimension dense, pointers 16-byte aligned; microscaled caches and scales dense.
+ */
+typedef struct dfx_split_attn_params {
+    const void* q;       /* [num_q_tokens, num_q_heads, head_dim] bf16 */
+    const void* k_new;   /* [num_new_tokens, num_kv_heads, head_dim] bf16 */
+    const void* v_new;
+    void* out;           /* [num_q_tokens, num_q_heads, head_dim] bf16 */
+    const void* k_cache; /* [n_pages, page_size, num_kv_heads, row]; NULL: no cached context */
+    const void* v_cache;
+    const void* k_scales; /* [n_pages, page_size, num_kv_heads, head_dim / 32] E8M0 bytes, DFX_KV_MX_* only */
+    const void* v_scales;
+    const int32_t* block_tables;   /* [num_seqs, block_table_stride] */
+    const int32_t* context_lens;   /* [num_seqs] */
+    const int32_t* cu_seqlens_q;   /* [num_seqs + 1] */
+    const int32_t* cu_seqlens_new; /* [num_seqs + 1] offsets of the fresh K/V rows */
+    const int32_t* prefix_cu_seqs; /* [num_groups + 1], ascending */
+    const int32_t* prefix_lens;    /* [num_groups] */
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_stride_token, q_stride_head;
+    int64_t kn_stride_token, kn_stride_head;
+    int64_t vn_stride_token, vn_stride_head;
+    int64_t o_stride_token, o_stride_head;
+    int64_t cache_stride_page, cache_stride_token, cache_stride_head; /* DFX_KV_BF16 */
+    int64_t block_table_stride;
+    int64_t n_pages;
+    int64_t num_q_tokens;   /* rows of q and out: none at or beyond it is touched, whatever the offsets say */
+    int64_t num_new_tokens; /* rows of k_new and v_new, likewise */
+    int32_t num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim;
+    int32_t page_size, max_pages_per_seq;
+    int32_t diffusion_block_size;
+    int32_t kv_dtype;       /* dfx_kv_dtype */
+    int32_t mask_mode;      /* dfx_mask_mode */
+    int32_t max_workgroups; /* 0: two per compute unit */
+    float scale;
+} dfx_split_attn_params;
+
+/* Negative: dfx_status.  Depends on num_seqs, num_groups, num_q_tokens, the head counts, head_dim and max_workgroups. */
+int64_t dfx_split_attn_workspace_bytes(const dfx_split_attn_params* params);
+int dfx_split_attn(const dfx_split_attn_params* params, dfx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
