@@ -96,7 +96,7 @@ class SplitAttnParams(C.Structure):
         ("num_seqs", C.c_int32), ("num_groups", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
         ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_pages_per_seq", C.c_int32),
         ("diffusion_block_size", C.c_int32), ("kv_dtype", C.c_int32), ("mask_mode", C.c_int32),
-        ("max_workgroups", C.c_int32), ("scale", C.c_float),
+        ("max_workgroups", C.c_int32), ("max_seqlen_q", C.c_int32), ("scale", C.c_float),
     ]
 
 

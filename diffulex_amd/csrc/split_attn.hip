@@ -9,16 +9,17 @@
 //
 // Work list: "virtual sequences" -- the groups (rows: all tokens of the group's sequences; keys: the prefix, through the first
 // sequence's block table) and then the sequences (keys: the context behind the prefix, then the fresh rows).  An item
-// is (virtual sequence, KV head, row tile), a unit one key tile of it; units have a cost and are dealt to the
-// workgroups in contiguous ranges of equal cost.  Every workgroup works the list out for itself from the lengths on the device (no
-// host read, safe in a captured graph with later lengths); a second launch merges the pieces.
+// is (virtual sequence, KV head or heads, row tile), a unit one key tile of it; items are dealt to the workgroups in
+// contiguous ranges of equal cost, cut where a range ends.  Every workgroup works the list out for itself from the lengths on the device (no
+// host read, safe in a captured graph with later lengths); the last launch merges the pieces.
 //
-// Two item kinds, chosen by the rows:
-//   narrow (rows <= 32: single tokens, small blocks): bound by memory.  Each of the four waves takes every fourth
-//     32-key tile into LDS of its own (no barrier in the loop, the next tile's loads in flight over the current one's
-//     arithmetic) and keeps a softmax state of its own; the four are merged in LDS at the end of the item.
-//   wide (more rows): bound by the matrix instructions and their LDS operands.  128 rows, 32 per wave, over 64-key tiles shared
-//     by the waves and double buffered.
+// Two kinds of items, chosen by the rows, each with a launch of its own (they want different register budgets):
+//   narrow (single tokens, small blocks): bound by memory.  32 rows; four waves, each with a KV head of its own where there are
+//     four (a token's codes and scales of neighbouring heads lie in the same memory lines: the waves of a workgroup should want them
+//     at the same time), with every second or fourth tile of a head otherwise, whose softmax states are then merged in LDS.
+//     A wave moves its 32-key tiles into LDS of its own: no barrier in the loop, the next tiles' loads in flight over the arithmetic.
+//   wide: bound by the matrix instructions and the exponentials.  256 rows, 32 for each of eight waves, over 64-key tiles shared by the
+//     waves; in each wave the products of one tile's scores run beside the exponentials of the tile before.
 // Microscaled codes are widened on the way from registers to LDS, once per tile, with their block's scale applied by the same
 // instruction: from there on the arithmetic is the bf16 cache's.
 #include "attn_tile.h"
@@ -27,13 +28,13 @@
 namespace dfx {
 namespace {
 
-constexpr int kWgThreads = 256;
-constexpr int kWgWaves = 4;
-constexpr int kNarrowRows = 32, kWideRows = 128;
+constexpr int kNarrowRows = 32, kWideRows = 256;
 constexpr int kNarrowKeys = 32, kWideKeys = 64;
-constexpr int kWideCost = 4;    // cost of a unit: a wide one takes a workgroup about as long as four narrow ones
-constexpr int kNarrowCost = 1;
-constexpr int kMinCost = 4;     // least cost per workgroup (>= the largest unit's: every range then holds a unit)
+constexpr int kNarrowMost = 96;  // rows of a virtual sequence up to which its items are narrow
+// Beside its units (cost 1 each) an item costs its start and end: queries, first tiles, the merge of the waves, the rows written.
+// (Narrow: of the tiles that the waves of a head take side by side; a unit is one such tile.)
+constexpr int kNarrowTail = 2, kWideTail = 3;
+constexpr int kNarrowLeast = 2, kWideLeast = 2;  // least cost per workgroup
 
 enum { kBf16 = 0, kMx8 = 1, kMx4 = 2 };
 
@@ -54,24 +55,29 @@ struct SplitArgs {
     const int32_t* group_len;
     uint8_t* workspace;
     int64_t q_st, q_sh, kn_st, kn_sh, vn_st, vn_sh, o_st, o_sh;
-    int64_t c_sp, c_st, c_sh;  // cache strides in bytes: page, token, head
+    uint32_t c_sp, c_st, c_sh;  // cache strides in bytes: page, token, head
     int64_t bt_stride;
-    int64_t tab_off, comb_off, slot_off, ml_off, n_slots;  // workspace
+    int64_t rec_off, comb_off, slot_off, ml_off;  // workspace
+    int64_t n_slots[2], first_slot[2];            // piece slots (32 rows each) of the narrow and the wide items
     int n_pages, n_q, n_new;
     int n_seqs, n_groups, h_kv, group_heads;
-    int page_size, page_shift, max_pages, dbs, block_causal, n_wg;
+    int page_size, page_shift, max_pages, dbs, block_causal, use_wide;
+    int n_wg[2];  // working workgroups of the narrow and the wide launch
+    int heads_shift;  // a narrow workgroup's KV heads: 1, 2 or 4 = 1 << heads_shift
     float c;  // scale * log2(e)
 };
 
-struct Header {
-    int64_t total;  // cost of all units
-    int32_t n_wg;   // workgroups that have work
-    int32_t n_comb; // row blocks of the merge
+struct Header {    // one per kind
+    int64_t total;   // cost of all items
+    int32_t n_wg;    // workgroups that have work
+    int32_t n_comb;  // row blocks of the merge (narrow launch)
 };
-struct TabEntry {
-    int64_t cost;  // of the units before the virtual sequence
-    int32_t blocks;  // row-block slots of the items before it
-    int32_t pad;
+struct Rec {         // a virtual sequence, for the merge
+    int64_t cost;    // of the items of its kind before it
+    int32_t blocks;  // row-block slots of the items of its kind before it
+    int32_t tok0, rows, tiles, row_tiles;
+    int32_t group;   // the group whose item covers a part of its keys, or -1
+    int32_t narrow, has_keys;
 };
 
 struct Seq {
@@ -83,22 +89,40 @@ struct Seq {
     int seq0, seq1;          // sequences of the item
     int tiles, ctx_tiles, row_tiles;
     bool narrow;
-    DFX_D int cost() const { return narrow ? kNarrowCost : kWideCost; }
-    DFX_D int row_blocks() const { return narrow ? 1 : kWideRows / 32; }  // slots of an item's piece
+    int group;               // its group, or -1
 };
+template <bool WIDE>
+struct Kind {
+    static constexpr int kWaves = WIDE ? 8 : 4, kThreads = kWaves * 64;
+};
+// What differs between the kinds and depends on the heads: the waves of a narrow workgroup that share a head take `side` tiles side by
+// side.
+struct Costs {
+    int tail, least;    // in tiles
+    int heads, blocks;  // KV heads of an item, slots of its pieces
+    DFX_D Costs(const SplitArgs& a, bool narrow) {
+        const int side = narrow ? Kind<false>::kWaves >> a.heads_shift : 1;
+        tail = narrow ? kNarrowTail * side : kWideTail;
+        least = narrow ? kNarrowLeast * side : kWideLeast;
+        heads = narrow ? 1 << a.heads_shift : 1;
+        blocks = narrow ? heads : kWideRows / 32;
+    }
+};
+// An item of `tiles` units: unit u starts at cost u, the tail's cost lies behind the last.
+DFX_D int item_cost(const Costs& k, int tiles) { return tiles > 0 ? tiles + k.tail : 0; }
 
 DFX_D int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-// Keys of sequence s's context that belong to its group's prefix.
-DFX_D int prefix_of(const SplitArgs& a, int s) {
-    int lo = 0, hi = a.n_groups;  // the last group that starts at or before s
-    if (hi == 0 || s < a.group_cu[0] || s >= a.group_cu[hi]) return 0;
-    while (hi - lo > 1) {
+// The group of sequence s, -1 if it is in none.
+DFX_D int group_of(const SplitArgs& a, int s) {
+    int lo = 0, hi = a.n_groups;
+    if (hi == 0 || s < a.group_cu[0] || s >= a.group_cu[hi]) return -1;
+    while (hi - lo > 1) {  // the last group that starts at or before s
         const int mid = (lo + hi) >> 1;
         if (a.group_cu[mid] <= s) lo = mid;
         else hi = mid;
     }
-    return max(a.group_len[lo], 0);
+    return lo;
 }
 
 DFX_D Seq seq_of(const SplitArgs& a, int v) {
@@ -106,6 +130,7 @@ DFX_D Seq seq_of(const SplitArgs& a, int v) {
     const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size;
     const int cap = static_cast<int>(capacity > INT32_MAX - 64 ? INT32_MAX - 64 : capacity);
     q.new0 = q.n_new = 0;
+    q.group = -1;
     if (v < a.n_groups) {
         q.seq0 = clampi(a.group_cu[v], 0, a.n_seqs);
         q.seq1 = clampi(a.group_cu[v + 1], q.seq0, a.n_seqs);
@@ -115,14 +140,15 @@ DFX_D Seq seq_of(const SplitArgs& a, int v) {
         q.seq0 = v - a.n_groups;
         q.seq1 = q.seq0 + 1;
         q.key1 = clampi(a.context_lens ? a.context_lens[q.seq0] : 0, 0, cap);
-        q.key0 = q.prefix = min(prefix_of(a, q.seq0), q.key1);
+        q.group = group_of(a, q.seq0);
+        q.key0 = q.prefix = q.group < 0 ? 0 : clampi(a.group_len[q.group], 0, q.key1);
         q.new0 = clampi(a.cu_new[q.seq0], 0, a.n_new);
         q.n_new = clampi(a.cu_new[q.seq1], q.new0, a.n_new) - q.new0;
     }
     q.table = q.seq0;
     q.tok0 = clampi(a.cu_q[q.seq0], 0, a.n_q);
     q.rows = (clampi(a.cu_q[q.seq1], q.tok0, a.n_q) - q.tok0) * a.group_heads;
-    q.narrow = q.rows <= kNarrowRows;
+    q.narrow = !a.use_wide || q.rows <= kNarrowMost;
     const int kt = q.narrow ? kNarrowKeys : kWideKeys, rt = q.narrow ? kNarrowRows : kWideRows;
     q.row_tiles = (q.rows + rt - 1) / rt;
     q.ctx_tiles = (q.key1 - q.key0 + kt - 1) / kt;
@@ -130,18 +156,28 @@ DFX_D Seq seq_of(const SplitArgs& a, int v) {
     return q;
 }
 
-// Workgroup ranges: workgroup w owns the units that start at a cost in [floor(w U / W), floor((w + 1) U / W)).
+// Workgroup ranges: workgroup w owns the units that start at a cost in [floor(w U / W), floor((w + 1) U / W)); so the owner of
+// cost x is floor(((x + 1) W - 1) / U).  (A quotient in fp64, put right: a 64-bit integer division is a hundred instructions.)
 DFX_D int64_t range_start(int w, int64_t total, int n_wg) { return w * total / n_wg; }
-DFX_D int owner_of(int64_t cost, int64_t total, int n_wg) { return static_cast<int>(((cost + 1) * n_wg - 1) / total); }
+DFX_D int owner_of(int64_t cost, int64_t total, int n_wg) {
+    const int64_t x = (cost + 1) * n_wg - 1;
+    int64_t q = static_cast<int64_t>(static_cast<double>(x) / static_cast<double>(total));
+    if (q * total > x) --q;
+    else if ((q + 1) * total <= x) ++q;
+    return static_cast<int>(q);
+}
 
-// ---- one wave's 32 rows ------------------------------------------------------------------------
-template <int HD>
+// ---- one wave's arithmetic ---------------------------------------------------------------------
+// NB blocks of 32 rows: lane (col, half) holds, of row col of each, the scores of keys 8 g + 4 half + (0..3) and the outputs
+// of elements d with the same pattern (S^T = K Q^T, O^T += V^T P^T: the probabilities leave the softmax in the layout the
+// second product's operand wants).
+template <int HD, int NB>
 struct Wave {
     using L = TileLayout<HD>;
     static constexpr int NSLAB = HD / 16, NDB = HD / 32;
-    f32x16 o[NDB];
-    bf16x8 q[NSLAB];
-    float m, l;
+    f32x16 o[NDB][NB];
+    bf16x8 q[NB][NSLAB];
+    float m[NB], l[NB];
     int lane, col, half;
     uint32_t k_lane, v_lane;
 
@@ -154,20 +190,23 @@ struct Wave {
     }
 
     DFX_D void reset() {
-        m = -INFINITY;
-        l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < NDB; ++d)
+        for (int b = 0; b < NB; ++b) {
+            m[b] = -INFINITY;
+            l[b] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][b][i] = 0.0f;
+        }
     }
 
-    DFX_D void load_q(const uint16_t* row) {  // nullptr: a lane without a row
+    DFX_D void load_q(int b, const uint16_t* row) {  // nullptr: a lane without a row
 #pragma unroll
         for (int s = 0; s < NSLAB; ++s) {
             u32x4 w = {0, 0, 0, 0};
             if (row != nullptr) w = *reinterpret_cast<const u32x4*>(row + s * 16 + half * 8);
-            q[s] = __builtin_bit_cast(bf16x8, w);
+            q[b][s] = __builtin_bit_cast(bf16x8, w);
         }
     }
 
@@ -190,273 +229,405 @@ struct Wave {
         return x + y;
     }
 
-    // S^T = K Q^T, softmax, O^T += V^T P^T over KT keys in LDS.  `seen`: this lane's visible keys, looked at where !full.
-    template <int KT>
-    DFX_D void tile(uint32_t kt, uint32_t vt, float c, bool full, uint64_t seen) {
-        constexpr int NT = KT / 32;
+    // Operands: 32 keys of one 16-wide slab of d; 16 keys (slab x of 32-key block t) of one 32-wide block of d, transposed.
+    DFX_D bf16x8 read_k(uint32_t kt, int t, int sl) const {
         typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
+        return *(const lds_bf16x8*)static_cast<uintptr_t>(((kt + k_lane) ^ (sl * 32)) + t * 32 * L::ROWB);
+    }
+    DFX_D bf16x8 read_v(uint32_t vt, int t, int x, int d) const {
         typedef short short4v __attribute__((ext_vector_type(4)));
-        typedef short short8v __attribute__((ext_vector_type(8)));
         typedef __attribute__((address_space(3))) short4v lds_short4v;
-        f32x16 s[NT];
+        short4v r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            r[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)static_cast<uintptr_t>(
+                ((vt + v_lane) ^ (((d * 4) ^ L::swizzle(i * 8)) * 16)) + (t * 32 + x * 16 + i * 8) * L::ROWB));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    template <int NT>
+    static DFX_D void clear(f32x16 (&s)[NT][NB]) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int sl = 0; sl < NSLAB; ++sl)
+                for (int i = 0; i < 16; ++i) s[t][b][i] = 0.0f;
+    }
+    template <int NT>
+    DFX_D void scores(uint32_t kt, f32x16 (&s)[NT][NB]) const {
+        constexpr int kAhead = 2;
+        clear(s);
+        bf16x8 k[kAhead + 1][NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const bf16x8 k = *(const lds_bf16x8*)static_cast<uintptr_t>(((kt + k_lane) ^ (sl * 32)) + t * 32 * L::ROWB);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[sl], s[t], 0, 0, 0);
+        for (int sl = 0; sl < NSLAB + kAhead; ++sl) {
+            if (sl < NSLAB) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) k[sl % (kAhead + 1)][t] = read_k(kt, t, sl);
             }
-        if (!full) {
+            if (sl >= kAhead) {
+                const int c = sl - kAhead;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t bits = static_cast<uint32_t>(seen >> (32 * t)) >> (4 * half);
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) s[t][i] = -INFINITY;
+                    for (int b = 0; b < NB; ++b) s[t][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[c % (kAhead + 1)][t], q[b][c], s[t][b], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);  // (all operands first would not fit the registers)
             }
         }
+    }
+
+    template <int NT>
+    DFX_D void hide(f32x16 (&s)[NT][NB], int b, uint64_t seen) const {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t bits = static_cast<uint32_t>(seen >> (32 * t)) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) s[t][b][i] = -INFINITY;
+        }
+    }
+
+    template <int NT>
+    DFX_D float top_of(const f32x16 (&s)[NT][NB], int b) const {
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-        top = half_max(top) * c;
-        // The running maximum moves only where a tile's is more than 2^8 above it (or there is none yet): the
-        // weights then stay below 2^8, far inside bf16 and fp32, and the accumulators are rarely rescaled.
-        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
-            const float next = fmaxf(m, top);
-            const float alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-            m = next;
-            l *= alpha;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][b][i]);
+        return top;
+    }
+
+    // The running maximum moves only where a tile's is more than 2^8 above it (or there is none yet): the
+    // weights then stay below 2^8, far inside bf16 and fp32, and the accumulators are rarely rescaled.
+    DFX_D void raise(int b, float top) {
+        if (__builtin_amdgcn_ballot_w64(top > m[b] + 8.0f)) {
+            const float next = fmaxf(m[b], top);
+            const float alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[b] - next);
+            m[b] = next;
+            l[b] *= alpha;
 #pragma unroll
             for (int d = 0; d < NDB; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                for (int i = 0; i < 16; ++i) o[d][b][i] *= alpha;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
-        bf16x8 p[NT][2];
+    }
+
+    DFX_D float base_of(int b) const { return m[b] == -INFINITY ? 0.0f : m[b]; }
+    // Weights of 16 keys (score registers 8 x .. 8 x + 7), rounded to bf16 for the second product; returns the sum of the
+    // unrounded ones.
+    static DFX_D float weights8(const f32x16& s, int x, float c, float base, bf16x8& p) {
+        float e[8];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float e[16];
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + i], c, -base));
+        u32x4 w;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -base));
-                l += e[i];
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{e[2 * i], e[2 * i + 1]}, bf16x2));
+        p = __builtin_bit_cast(bf16x8, w);
+        return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    }
+    template <int NT>
+    DFX_D void weights(const f32x16 (&s)[NT][NB], float c, bf16x8 (&p)[NB][NT][2]) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float base = base_of(b);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) l[b] += weights8(s[t][b], x, c, base, p[b][t][x]);
+        }
+    }
+
+    template <int NT>
+    DFX_D void accumulate(uint32_t vt, const bf16x8 (&p)[NB][NT][2]) {
+        constexpr int kSteps = 2 * NT * NDB, kAhead = 3;
+        bf16x8 v[kAhead + 1];
+#pragma unroll
+        for (int st = 0; st < kSteps + kAhead; ++st) {
+            if (st < kSteps) v[st % (kAhead + 1)] = read_v(vt, st / (2 * NDB), (st / NDB) & 1, st % NDB);
+            if (st >= kAhead) {
+                const int c = st - kAhead, t = c / (2 * NDB), x = (c / NDB) & 1, d = c % NDB;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[d][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[c % (kAhead + 1)], p[b][t][x], o[d][b], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+    // The two halves of a wide tile's step, with the vector work of one tile between the matrix instructions of another and
+    // the LDS operands requested some instructions ahead: an operand takes longer to arrive than a matrix instruction to run.
+    // The scheduling barriers keep the source's order: left to itself the compiler puts the matrix instructions in a row (a wave waits at
+    // the second until the first is through the pipeline), or all loads first, which does not fit the registers.
+    static constexpr int kAheadK = 2;  // slabs
+    static constexpr int kAheadV = 3;  // 16 keys x 32 elements each
+    //   weights of s, scores of the next tile, and the first operands of the second half
+    DFX_D void weights_and_scores(const f32x16 (&s)[2][NB], float c, bf16x8 (&p)[NB][2][2], uint32_t kt, f32x16 (&next)[2][NB], uint32_t vt,
+                                  bf16x8 (&v)[kAheadV + 1]) {
+        static_assert(NB == 1, "the weights of a slab's step are those of one row block");
+        constexpr int kEach = 32 / NSLAB;  // weights per step
+        clear(next);
+        const float base = base_of(0);
+        float sum = 0.0f;
+        uint32_t w[2][8];  // pairs of weights
+        bf16x8 k[kAheadK + 1][2];
+#pragma unroll
+        for (int sl = 0; sl < kAheadK; ++sl) {
+            k[sl][0] = read_k(kt, 0, sl);
+            k[sl][1] = read_k(kt, 1, sl);
+        }
+#pragma unroll
+        for (int sl = 0; sl < NSLAB; ++sl) {
+            if (sl + kAheadK < NSLAB) {
+                k[(sl + kAheadK) % (kAheadK + 1)][0] = read_k(kt, 0, sl + kAheadK);
+                k[(sl + kAheadK) % (kAheadK + 1)][1] = read_k(kt, 1, sl + kAheadK);
+            } else {
+#pragma unroll
+                for (int i = (sl + kAheadK - NSLAB) * kAheadV / kAheadK; i < (sl + kAheadK - NSLAB + 1) * kAheadV / kAheadK; ++i)
+                    v[i] = read_v(vt, i / (2 * NDB), (i / NDB) & 1, i % NDB);
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                u32x4 w;
+            for (int i = 0; i < 2; ++i) {
+                next[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[sl % (kAheadK + 1)][i], q[0][sl], next[i][0], 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{e[8 * x + 2 * i], e[8 * x + 2 * i + 1]}, bf16x2));
-                p[t][x] = __builtin_bit_cast(bf16x8, w);
+                for (int j = 0; j < kEach / 2; j += 2) {
+                    const int e = sl * kEach + i * (kEach / 2) + j, t = e >> 4;
+                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][0][e & 15], c, -base));
+                    const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][0][(e & 15) + 1], c, -base));
+                    sum += w0 + w1;
+                    w[t][(e & 15) >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{w0, w1}, bf16x2));
+                    // (wanted here: otherwise they are all made behind the last matrix instruction)
+                    asm volatile("" : "+v"(w[t][(e & 15) >> 1]), "+v"(sum));
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        l[0] += sum;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
+                p[0][t][x] = __builtin_bit_cast(bf16x8, u32x4{w[t][4 * x], w[t][4 * x + 1], w[t][4 * x + 2], w[t][4 * x + 3]});
+    }
+    //   outputs of a tile and the largest of the next tile's scores (this half's, unscaled)
+    DFX_D void accumulate_and_top(uint32_t vt, const bf16x8 (&p)[NB][2][2], const f32x16 (&next)[2][NB], float (&top)[NB],
+                                  bf16x8 (&v)[kAheadV + 1]) {
+        constexpr int kSteps = 4 * NDB;
+        constexpr int kEach = 32 / kSteps;  // scores per step
+        top[0] = -INFINITY;
 #pragma unroll
-                for (int d = 0; d < NDB; ++d) {
-                    short4v r[2];
+        for (int st = 0; st < kSteps; ++st) {
+            const int t = st / (2 * NDB), x = (st / NDB) & 1, d = st % NDB, n = st + kAheadV;
+            if (n < kSteps) v[n % (kAheadV + 1)] = read_v(vt, n / (2 * NDB), (n / NDB) & 1, n % NDB);
+            o[d][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[st % (kAheadV + 1)], p[0][t][x], o[d][0], 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        r[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_short4v*)static_cast<uintptr_t>(((vt + v_lane) ^ (((d * 4) ^ L::swizzle(i * 8)) * 16)) +
-                                                                 (t * 32 + x * 16 + i * 8) * L::ROWB));
-                    const short8v v = __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), p[t][x], o[d], 0, 0, 0);
-                }
+            for (int i = 0; i < kEach; ++i) top[0] = fmaxf(top[0], next[(st * kEach + i) >> 4][0][(st * kEach + i) & 15]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 };
 
 DFX_D void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// ---- a workgroup's walk over its units ---------------------------------------------------------
-template <int HD, int KV>
+// ---- a workgroup's items -----------------------------------------------------------------------
+template <int HD, int KV, bool WIDE>
 struct Split {
     using L = TileLayout<HD>;
-    using W = Wave<HD>;
+    static constexpr int NB = 1;  // row blocks of a wave
+    static constexpr int kWgWaves = Kind<WIDE>::kWaves, kWgThreads = Kind<WIDE>::kThreads;
+    using W = Wave<HD, NB>;
     static constexpr int NDB = HD / 32;
     static constexpr int kRowBytes = KV == kBf16 ? HD * 2 : KV == kMx8 ? HD : HD / 2;  // codes of a head row
     static constexpr int kChunks = kRowBytes / 16;                                     // 16-byte chunks of them
     static constexpr int kNewChunks = HD / 8;                                          // of a fresh (bf16) row
-    static constexpr int kTileBytes = kWideKeys * L::ROWB;
-    static constexpr int kLds = 4 * kTileBytes;  // wide: two buffers of K and V; narrow: K and V of 32 keys per wave
+    static constexpr int KT = WIDE ? kWideKeys : kNarrowKeys;
+    static constexpr int ROWS = WIDE ? kWideKeys / kWgWaves : kNarrowKeys;             // rows of a tile that one wave moves
+    static constexpr int kMat = KT * L::ROWB;                                          // K or V of a tile in LDS
+    static constexpr int kLds = WIDE ? 4 * kMat : kWgWaves * 2 * kMat;                 // two buffers each; a tile per wave
     static constexpr int kAccBytes = 32 * HD * 4;
+    static constexpr int kPer = 64 / kChunks;                                          // rows per load of the wave
+    static constexpr int kLoads = ROWS > kPer ? ROWS / kPer : 1;                       // (one that some lanes only repeat, where ROWS < kPer)
+    // Tiles in flight per wave of a narrow item.  The eight waves of a compute unit should have some 100 KB on the way; a bf16
+    // tile is 16 KB.
+    static constexpr int kDepth = KV == kBf16 ? 1 : KV == kMx8 ? 2 : 3;
+    static constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << 32) - 1;
 
     const SplitArgs& a;
     uint8_t* lds;
-    float* ml;     // [4 waves][m, l][32]
+    float* ml;  // [4 waves][m, l][32]
     int tid, wave, lane;
     W w;
     // the item
     Seq sq;
     int kvh, row_tile;
-    int lim_ctx, lim_new;      // this lane's row sees cached keys below lim_ctx and fresh rows below lim_new
-    int64_t head_off;
+    int lim_ctx[NB], lim_new[NB];  // this lane's rows see cached keys below lim_ctx and fresh rows below lim_new
+    uint64_t lane_off;             // of the KV head and of this lane's chunk, in a cache row
 
     DFX_D Split(const SplitArgs& args, uint8_t* smem, float* ml_, int tid_)
         : a(args), lds(smem), ml(ml_), tid(tid_), wave(uniform(tid_ >> 6)), lane(tid_ & 63), w(tid_ & 63) {}
 
-    // Cache slot byte offset of key position pos (this lane's), -1 where there is none.
-    DFX_D int64_t row_of(int pos) const {
-        if (pos >= sq.key1) return -1;
+    // Key `lane` of tile t: look_up() loads its page's table entry, row_of() -- a tile later, so that nothing waits for the load --
+    // makes it the byte offset of the key's cache row (token) and tells which keys have none: fresh tiles, keys behind the last,
+    // skipped pages (offset 0: the cache's first row).
+    struct Key {
+        int page, off;
+        bool ok;
+    };
+    DFX_D Key look_up(int t) const {
+        const int pos = sq.key0 + t * KT + lane;
         const int p = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
-        if (p >= a.max_pages) return -1;
-        const int page = a.block_tables[sq.table * a.bt_stride + p];
-        if (page < 0 || page >= a.n_pages) return -1;
-        return page * a.c_sp + (pos - p * a.page_size) * a.c_st;
+        Key k;
+        k.ok = t < sq.ctx_tiles && lane < KT && pos < sq.key1 && p < a.max_pages;
+        k.off = pos - p * a.page_size;
+        k.page = a.block_tables[sq.table * a.bt_stride + min(p, a.max_pages - 1)];
+        return k;
+    }
+    DFX_D int64_t row_of(const Key& k, uint64_t& valid) const {
+        const bool ok = k.ok && k.page >= 0 && k.page < a.n_pages;
+        valid = __builtin_amdgcn_ballot_w64(ok);
+        const uint32_t page = ok ? k.page : 0, off = ok ? k.off : 0;
+        return static_cast<int64_t>(static_cast<uint64_t>(page) * a.c_sp + static_cast<uint64_t>(off) * a.c_st);
     }
 
-    // Rows of a KT-key tile that one wave moves: all of them (narrow) or its quarter (wide).
-    template <int KT, int ROWS>
+    // The wave's share of a K or V tile on its way: loads i, rows r0 + stage_row(i), chunk lane % kChunks.
     struct Stage {
-        static constexpr int kPer = 64 / kChunks > ROWS ? ROWS : 64 / kChunks;        // rows per load of the wave
-        static constexpr int kLoads = ROWS / kPer;
-        u32x4 k[kLoads], v[kLoads];
-        uint8_t ks[kLoads], vs[kLoads];
-        uint64_t valid;  // keys of the tile that have a cache row
-        bool fresh;
+        u32x4 w[kLoads];
+        uint8_t s[kLoads];
     };
-
+    // Which of a load's rows a lane takes.  A chunk of codes becomes 2 or 4 chunks in LDS, which leave one per lane at a time: 16 lanes
+    // should then write all 16 chunk positions of a 256-byte LDS line, i.e. lie on rows whose swizzles (TileLayout) differ where their
+    // chunk indices agree, in the lowest bits -- that is row bits 2 and 3.
+    static DFX_D int lane_row(int j) {
+        if constexpr (KV == kBf16) return j;
+        if constexpr (HD == 128 && KV == kMx8) return ((j & 1) << 2) | (j >> 1);                                   // of 8
+        if constexpr (HD == 128 && KV == kMx4) return ((j & 3) << 2) | (j >> 2);                                   // of 16
+        if constexpr (HD == 64 && KV == kMx8) return (j & 9) | ((j & 2) << 1) | ((j & 4) >> 1);                    // of 16
+        return (j & 17) | ((j & 2) << 1) | ((j & 4) << 1) | ((j & 8) >> 2);                                        // of 32
+    }
+    DFX_D int stage_row(int i) const { return i * kPer + lane_row(lane / kChunks); }
     static DFX_D int64_t shuffle64(int64_t x, int from) {
         const int lo = __builtin_amdgcn_ds_bpermute(from * 4, static_cast<int>(x));
         const int hi = __builtin_amdgcn_ds_bpermute(from * 4, static_cast<int>(x >> 32));
         return static_cast<int64_t>(static_cast<uint32_t>(lo)) | (static_cast<int64_t>(hi) << 32);
     }
-
-    // row: lane l's cache row of key l of the tile (row_of).  Issues the loads of the wave's rows [r0, r0 + ROWS).
-    template <int KT, int ROWS>
-    DFX_D void issue(Stage<KT, ROWS>& st, int64_t row, int r0) const {
-        using S = Stage<KT, ROWS>;
-        st.fresh = false;
-        st.valid = __builtin_amdgcn_ballot_w64(row >= 0);
+    // Issues the loads; `row` is row_of() the tile's keys.  No branch on the rows -- keys without a cache row load the cache's first
+    // row and are zeroed in commit() -- so that the compiler can count the loads in flight.
+    DFX_D void issue(Stage& st, const uint8_t* codes, const uint8_t* scales, int64_t row, int r0) const {
 #pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-            const int r = i * S::kPer + lane / kChunks, ch = lane % kChunks;
-            const int64_t at = shuffle64(row, r0 + (r < ROWS ? r : 0));
-            st.k[i] = st.v[i] = u32x4{0, 0, 0, 0};
-            st.ks[i] = st.vs[i] = 0;
-            if (at >= 0 && r < ROWS) {
-                const int64_t off = at + head_off + ch * 16;
-                st.k[i] = *reinterpret_cast<const u32x4*>(a.k_cache + off);
-                st.v[i] = *reinterpret_cast<const u32x4*>(a.v_cache + off);
-                if constexpr (KV != kBf16) {
-                    const int64_t so = off / (KV == kMx8 ? 32 : 16);
-                    st.ks[i] = a.k_scales[so];
-                    st.vs[i] = a.v_scales[so];
-                }
-            }
+        for (int i = 0; i < kLoads; ++i) {
+            const uint64_t off = static_cast<uint64_t>(shuffle64(row, r0 + min(stage_row(i), ROWS - 1))) + lane_off;
+            st.w[i] = *reinterpret_cast<const u32x4*>(codes + off);
+            if constexpr (KV != kBf16) st.s[i] = scales[off >> (KV == kMx8 ? 5 : 4)];
         }
     }
-
-    // Registers -> LDS, widened.
-    template <int KT, int ROWS>
-    DFX_D void commit(const Stage<KT, ROWS>& st, uint8_t* kt, uint8_t* vt, int r0) const {
-        using S = Stage<KT, ROWS>;
+    // Registers -> LDS, widened.  valid: which keys of the tile have a cache row.
+    DFX_D void commit(Stage& st, uint8_t* to, int r0, uint64_t valid) const {
+        if (valid != kAll) {  // (a wave-uniform branch)
 #pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-            const int r = i * S::kPer + lane / kChunks, ch = lane % kChunks;
-            if (S::kPer * kChunks < 64 && r >= ROWS) continue;
+            for (int i = 0; i < kLoads; ++i)
+                if (!((valid >> ((r0 + stage_row(i)) & 63)) & 1)) {
+                    st.w[i] = u32x4{0, 0, 0, 0};
+                    st.s[i] = 0;
+                }
+        }
+        int j = lane;
+        asm volatile("" : "+v"(j));  // (addresses worked out here: as invariants of the tile loop they take the registers of its tiles)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = i * kPer + lane_row(j / kChunks), ch = j % kChunks;
+            if (ROWS < kPer && r >= ROWS) continue;
             if constexpr (KV == kBf16) {
-                const int off = L::chunk_offset(r0 + r, ch);
-                *reinterpret_cast<u32x4*>(kt + off) = st.k[i];
-                *reinterpret_cast<u32x4*>(vt + off) = st.v[i];
+                *reinterpret_cast<u32x4*>(to + L::chunk_offset(r0 + r, ch)) = st.w[i];
             } else {
-                const float ks = mx_scale_operand(st.ks[i]), vs = mx_scale_operand(st.vs[i]);
+                const float s = mx_scale_operand(st.s[i]);
                 constexpr int N = KV == kMx8 ? 2 : 4;
 #pragma unroll
                 for (int x = 0; x < N; ++x) {
-                    const int off = L::chunk_offset(r0 + r, ch * N + x);
-                    if constexpr (KV == kMx8) {
-                        *reinterpret_cast<u32x4*>(kt + off) = mx_widen8_e4m3(u32x2{st.k[i][2 * x], st.k[i][2 * x + 1]}, ks);
-                        *reinterpret_cast<u32x4*>(vt + off) = mx_widen8_e4m3(u32x2{st.v[i][2 * x], st.v[i][2 * x + 1]}, vs);
-                    } else {
-                        *reinterpret_cast<u32x4*>(kt + off) = mx_widen8_e2m1(st.k[i][x], ks);
-                        *reinterpret_cast<u32x4*>(vt + off) = mx_widen8_e2m1(st.v[i][x], vs);
-                    }
+                    u32x4 y;
+                    if constexpr (KV == kMx8) y = mx_widen8_e4m3(u32x2{st.w[i][2 * x], st.w[i][2 * x + 1]}, s);
+                    else y = mx_widen8_e2m1(st.w[i][x], s);
+                    *reinterpret_cast<u32x4*>(to + L::chunk_offset(r0 + r, ch * N + x)) = y;
                 }
             }
         }
     }
-
-    // Fresh rows [j0, j0 + KT) (bf16 operands): straight to LDS, there are few of them.
-    template <int ROWS>
-    DFX_D void fresh_rows(int j0, uint8_t* kt, uint8_t* vt, int r0) const {
-        constexpr int kPer = 64 / kNewChunks;
+    // Fresh rows (bf16 operands) of fresh tile t: straight to LDS, there are few of them.
+    DFX_D void fresh_rows(const uint16_t* from, int64_t st, int64_t sh, int t, uint8_t* to, int r0) const {
+        constexpr int kStep = 64 / kNewChunks;
 #pragma unroll
-        for (int i = 0; i < ROWS / kPer; ++i) {
-            const int r = r0 + i * kPer + lane / kNewChunks, ch = lane % kNewChunks;
-            u32x4 kk = {0, 0, 0, 0}, vv = {0, 0, 0, 0};
-            if (j0 + r < sq.n_new) {
-                const int64_t t = sq.new0 + j0 + r;
-                kk = *reinterpret_cast<const u32x4*>(a.k_new + t * a.kn_st + kvh * a.kn_sh + ch * 8);
-                vv = *reinterpret_cast<const u32x4*>(a.v_new + t * a.vn_st + kvh * a.vn_sh + ch * 8);
-            }
-            const int off = L::chunk_offset(r, ch);
-            *reinterpret_cast<u32x4*>(kt + off) = kk;
-            *reinterpret_cast<u32x4*>(vt + off) = vv;
+        for (int i = 0; i < ROWS / kStep; ++i) {
+            const int r = r0 + i * kStep + lane / kNewChunks, ch = lane % kNewChunks, j = t * KT + r;
+            u32x4 x = {0, 0, 0, 0};
+            if (j < sq.n_new) x = *reinterpret_cast<const u32x4*>(from + (sq.new0 + static_cast<int64_t>(j)) * st + kvh * sh + ch * 8);
+            *reinterpret_cast<u32x4*>(to + L::chunk_offset(r, ch)) = x;
         }
     }
-
     static DFX_D uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
+    static DFX_D uint32_t address(const uint8_t* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); }
 
-    template <int KT>
-    DFX_D void compute(const uint8_t* kt, const uint8_t* vt, int t, uint64_t valid) {
-        const bool fresh = t >= sq.ctx_tiles;
-        const int base = fresh ? (t - sq.ctx_tiles) * KT : sq.key0 + t * KT;
-        const int visible = (fresh ? lim_new : lim_ctx) - base;
-        const uint64_t all = KT == 64 ? ~0ull : (1ull << 32) - 1;
-        const bool full = (fresh || (valid & all) == all) && __builtin_amdgcn_ballot_w64(visible < KT) == 0;
-        w.template tile<KT>(TileMathAddress(kt), TileMathAddress(vt), a.c, full, below(visible) & (fresh ? ~0ull : valid));
+    // Scores of the keys that a row does not see: of context tile t, of fresh tile t (counted from the first fresh one).
+    template <int NT>
+    DFX_D void mask_context(f32x16 (&s)[NT][NB], int t, uint64_t valid) const {
+        const int visible = lim_ctx[0] - (sq.key0 + t * KT);
+        if (valid == kAll && __builtin_amdgcn_ballot_w64(visible < KT) == 0) return;
+        w.hide(s, 0, below(visible) & valid);
     }
-    static DFX_D uint32_t TileMathAddress(const uint8_t* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); }
-
-    DFX_D int64_t lane_row(int t, int kt) const {  // row of key `lane` of context tile t, -1 for fresh tiles
-        return t < sq.ctx_tiles && lane < kt ? row_of(sq.key0 + t * kt + lane) : -1;
+    template <int NT>
+    DFX_D void mask_fresh(f32x16 (&s)[NT][NB], int t) const {
+        const int visible = lim_new[0] - t * KT;
+        if (__builtin_amdgcn_ballot_w64(visible < KT) == 0) return;
+        w.hide(s, 0, below(visible));
+    }
+    // All of a tile's arithmetic.
+    template <typename Mask>
+    DFX_D void whole_tile(const uint8_t* kt, const uint8_t* vt, const Mask& mask) {
+        constexpr int NT = KT / 32;
+        f32x16 s[NT][NB];
+        bf16x8 p[NB][NT][2];
+        w.scores(address(kt), s);
+        mask(s);
+        w.raise(0, W::half_max(w.top_of(s, 0)) * a.c);
+        w.weights(s, a.c, p);
+        w.accumulate(address(vt), p);
     }
 
-    DFX_D void start_item(int rows_from) {
-        head_off = kvh * a.c_sh;
-        const int row = rows_from + w.col;
+    // (one block of rows after the other, not a loop over them: a loop that holds another is unrolled too late for the compiler to
+    // keep the state it indexes in registers)
+    DFX_D void start_rows(int b, int rows_from, bool uneven) {
+        const int row = rows_from + b * 32 + w.col;
         const bool live = row < sq.rows;
         const int t = live ? row / a.group_heads : 0, g = live ? row - t * a.group_heads : 0;
         const int64_t tok = sq.tok0 + t;
-        w.load_q(live ? a.q + tok * a.q_st + (static_cast<int64_t>(kvh) * a.group_heads + g) * a.q_sh : nullptr);
-        w.reset();
-        lim_ctx = live ? sq.key1 : INT32_MAX;
-        lim_new = !live ? INT32_MAX : a.block_causal ? min(sq.n_new, (t / a.dbs + 1) * a.dbs) : sq.n_new;
-    }
-
-    // A group's rows whose sequence's context ends inside the prefix (or before it) see less of it.
-    DFX_D void limit_rows(int rows_from) {
-        const int row = rows_from + w.col;
-        if (row >= sq.rows) return;
-        const int tok = sq.tok0 + row / a.group_heads;
-        int lo = sq.seq0, hi = sq.seq1;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.cu_q[mid] <= tok) lo = mid;
-            else hi = mid;
+        w.load_q(b, live ? a.q + tok * a.q_st + (static_cast<int64_t>(kvh) * a.group_heads + g) * a.q_sh : nullptr);
+        int ctx = live ? sq.key1 : INT32_MAX;
+        if (uneven && live) {  // the row's sequence may end inside the prefix, or before it
+            int lo = sq.seq0, hi = sq.seq1;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.cu_q[mid] <= tok) lo = mid;
+                else hi = mid;
+            }
+            ctx = min(sq.key1, max(a.context_lens[lo], 0));
         }
-        lim_ctx = min(sq.key1, max(a.context_lens ? a.context_lens[lo] : 0, 0));
+        lim_ctx[b] = ctx;
+        lim_new[b] = !live ? INT32_MAX : a.block_causal ? min(sq.n_new, (t / a.dbs + 1) * a.dbs) : sq.n_new;
+    }
+    DFX_D void start_item(int rows_from, bool is_group) {
+        lane_off = kvh * static_cast<uint64_t>(a.c_sh) + lane % kChunks * 16;
+        const bool uneven = uneven_group(is_group);
+        w.reset();
+        start_rows(0, rows_from, uneven);
+        if constexpr (NB > 1) start_rows(1, rows_from, uneven);
     }
     DFX_D bool uneven_group(bool is_group) {
         if (!is_group) return false;
         bool any = false;
-        for (int s = sq.seq0 + tid; s < sq.seq1; s += kWgThreads) any |= (a.context_lens ? a.context_lens[s] : 0) < sq.key1;
+        for (int s = sq.seq0 + tid; s < sq.seq1; s += kWgThreads) any |= a.context_lens[s] < sq.key1;
         return __syncthreads_or(any);
     }
 
     DFX_D float* acc_slot(int64_t slot) const { return reinterpret_cast<float*>(a.workspace + a.slot_off + slot * kAccBytes); }
     DFX_D float* ml_slot(int64_t slot) const { return reinterpret_cast<float*>(a.workspace + a.ml_off) + slot * 64; }
+    DFX_D bool has_slot(int64_t slot) const { return slot < a.first_slot[WIDE] + a.n_slots[WIDE]; }
 
-    // d block `d` of a row block: a piece to its slot, or the finished rows to the output.
+    // d block `d` of the row block from row rows_from on: a piece to its slot, or the finished rows to the output.
     DFX_D void put(f32x16 o, int d, float inv, int rows_from, int64_t slot, bool direct) {
         const int row = rows_from + w.col;
         if (row >= sq.rows) return;
@@ -478,333 +649,454 @@ struct Split {
     }
 
     // ---- wide ----------------------------------------------------------------------------------
+    // Context tiles: K runs a tile ahead of V; while the weights of tile u are made, the matrix pipeline makes the scores of
+    // u + 1.  Registers hold K of u + 2 and V of u + 1 on their way to LDS, the cache rows of u + 2 are known, those of u + 3 looked up.
+    // No branch on the tile's kind in the loop and every wait for a step's loads before the next are issued: where a wait can be reached
+    // with other loads in flight, the compiler waits for all of them.
     DFX_D void wide(int u0, int u1, bool is_group, int64_t slot, bool direct) {
-        using S = Stage<kWideKeys, kWideKeys / kWgWaves>;
-        constexpr int ROWS = kWideKeys / kWgWaves;
         const int rows_from = row_tile * kWideRows + wave * 32;
-        const bool uneven = uneven_group(is_group);
-        start_item(rows_from);
-        if (uneven) limit_rows(rows_from);
+        start_item(rows_from, is_group);
+        const bool busy = rows_from < sq.rows;
         const int r0 = wave * ROWS;
-        S st;
-        uint64_t valid = 0;
-        int64_t row = lane_row(u0, kWideKeys);
-        issue(st, row, r0);
-        row = u0 + 1 < u1 ? lane_row(u0 + 1, kWideKeys) : -1;
-        for (int u = u0; u < u1; ++u) {
-            uint8_t* kt = lds + ((u - u0) & 1) * 2 * kTileBytes;
-            uint8_t* vt = kt + kTileBytes;
-            if (u < sq.ctx_tiles) commit(st, kt, vt, r0);
-            else fresh_rows<ROWS>((u - sq.ctx_tiles) * kWideKeys, kt, vt, r0);
-            valid = st.valid;
-            if (u + 1 < u1) {
-                issue(st, row, r0);
-                row = u + 2 < u1 ? lane_row(u + 2, kWideKeys) : -1;
+        auto k_buf = [&](int u) { return lds + ((u - u0) & 1) * kMat; };
+        auto v_buf = [&](int u) { return lds + (2 + ((u - u0) & 1)) * kMat; };
+        const int c1 = min(u1, sq.ctx_tiles);
+        if (u0 < c1) {
+            Stage sk, sv;
+            f32x16 s[2][NB];
+            float top[NB];
+            int64_t row2;                     // cache rows of tile u + 2
+            Key key3;                         // keys of tile u + 3
+            uint64_t valid0, valid1, valid2;  // keys with a cache row of tiles u, u + 1, u + 2
+            {
+                const Key key0 = look_up(u0), key1 = look_up(u0 + 1), key2 = look_up(u0 + 2);
+                key3 = look_up(u0 + 3);
+                const int64_t row0 = row_of(key0, valid0), row1 = row_of(key1, valid1);
+                row2 = row_of(key2, valid2);
+                issue(sk, a.k_cache, a.k_scales, row0, r0);
+                issue(sv, a.v_cache, a.v_scales, row0, r0);
+                commit(sk, k_buf(u0), r0, valid0);
+                issue(sk, a.k_cache, a.k_scales, row1, r0);
+                commit(sv, v_buf(u0), r0, valid0);
+                issue(sv, a.v_cache, a.v_scales, row1, r0);
             }
             lds_barrier();
-            compute<kWideKeys>(kt, vt, u, valid);
-        }
-        if (rows_from < sq.rows) {
-            const float l = W::half_sum(w.l);
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            const bool fits = slot + wave < a.n_slots;
-            if (direct || fits) {
-#pragma unroll
-                for (int d = 0; d < NDB; ++d) put(w.o[d], d, inv, rows_from, slot + wave, direct);
-                if (!direct) ml_slot(slot + wave)[lane] = w.half ? l : w.m;
+            if (busy) {
+                w.scores(address(k_buf(u0)), s);
+                mask_context(s, u0, valid0);
+                top[0] = W::half_max(w.top_of(s, 0)) * a.c;
+            }
+            commit(sk, k_buf(u0 + 1), r0, valid1);
+            issue(sk, a.k_cache, a.k_scales, row2, r0);
+            lds_barrier();
+            for (int u = u0; u + 1 < c1; ++u) {
+                const Key key4 = look_up(u + 4);
+                if (busy) {
+                    bf16x8 p[NB][2][2];
+                    f32x16 next[2][NB];
+                    w.raise(0, top[0]);
+                    bf16x8 v[W::kAheadV + 1];
+                    w.weights_and_scores(s, a.c, p, address(k_buf(u + 1)), next, address(v_buf(u)), v);
+                    mask_context(next, u + 1, valid1);
+                    w.accumulate_and_top(address(v_buf(u)), p, next, top, v);
+                    top[0] = W::half_max(top[0]) * a.c;
+                    s[0][0] = next[0][0];
+                    s[1][0] = next[1][0];
+                }
+                commit(sv, v_buf(u + 1), r0, valid1);
+                commit(sk, k_buf(u), r0, valid2);  // (of tile u + 2; behind the last, zeros that nobody reads)
+                issue(sv, a.v_cache, a.v_scales, row2, r0);
+                valid1 = valid2;
+                row2 = row_of(key3, valid2);
+                issue(sk, a.k_cache, a.k_scales, row2, r0);
+                key3 = key4;
+                lds_barrier();
+            }
+            if (busy) {
+                bf16x8 p[NB][2][2];
+                w.raise(0, top[0]);
+                w.weights(s, a.c, p);
+                w.accumulate(address(v_buf(c1 - 1)), p);
             }
         }
+        for (int u = max(u0, sq.ctx_tiles); u < u1; ++u) {
+            const int t = u - sq.ctx_tiles;
+            lds_barrier();
+            fresh_rows(a.k_new, a.kn_st, a.kn_sh, t, lds, r0);
+            fresh_rows(a.v_new, a.vn_st, a.vn_sh, t, lds + kMat, r0);
+            lds_barrier();
+            if (busy) whole_tile(lds, lds + kMat, [&](auto& s) { mask_fresh(s, t); });
+        }
         lds_barrier();  // (the next item's tiles)
+        if (busy && (direct || has_slot(slot + wave))) {
+            const float l = W::half_sum(w.l[0]);
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, rows_from, slot + wave, direct);
+            if (!direct) ml_slot(slot + wave)[lane] = w.half ? l : w.m[0];
+        }
     }
 
     // ---- narrow --------------------------------------------------------------------------------
     DFX_D void narrow(int u0, int u1, bool is_group, int64_t slot, bool direct) {
-        using S = Stage<kNarrowKeys, kNarrowKeys>;
-        uint8_t* kt = lds + wave * 2 * (kNarrowKeys * L::ROWB);
-        uint8_t* vt = kt + kNarrowKeys * L::ROWB;
-        const bool uneven = uneven_group(is_group);
-        start_item(row_tile * kNarrowRows);
-        if (uneven) limit_rows(row_tile * kNarrowRows);
-        S st;
-        const int first = u0 + wave;
-        int64_t row = first < u1 ? lane_row(first, kNarrowKeys) : -1;
-        if (first < u1) issue(st, row, 0);
-        row = first + kWgWaves < u1 ? lane_row(first + kWgWaves, kNarrowKeys) : -1;
-        for (int u = first; u < u1; u += kWgWaves) {
-            if (u < sq.ctx_tiles) commit(st, kt, vt, 0);
-            else fresh_rows<kNarrowKeys>((u - sq.ctx_tiles) * kNarrowKeys, kt, vt, 0);
-            const uint64_t valid = st.valid;
-            if (u + kWgWaves < u1) {
-                issue(st, row, 0);
-                row = u + 2 * kWgWaves < u1 ? lane_row(u + 2 * kWgWaves, kNarrowKeys) : -1;
+        uint8_t* kt = lds + wave * 2 * kMat;
+        uint8_t* vt = kt + kMat;
+        // wave = head of the group * side + place among the head's waves
+        const int side_shift = 2 - a.heads_shift, side = 1 << side_shift;
+        const int my_head = wave >> side_shift;
+        kvh = (kvh << a.heads_shift) + my_head;
+        slot += my_head;
+        start_item(row_tile * kNarrowRows, is_group);
+        int u = u0 + (wave & (side - 1));
+        const int c1 = min(u1, sq.ctx_tiles);
+        if (u < c1) {
+            Stage sk[kDepth], sv[kDepth];
+            uint64_t valid[kDepth];
+            // A table entry is looked up kDepth tiles before its rows' loads are issued, so that it is in front of the loads that a tile's
+            // commit waits for: loads return in order, and a wait for a younger entry would drain the tiles in flight.
+            Key keys[kDepth];
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i) keys[i] = look_up(u + i * side);
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i) {
+                const int64_t row = row_of(keys[i], valid[i]);
+                keys[i] = look_up(u + (kDepth + i) * side);
+                issue(sk[i], a.k_cache, a.k_scales, row, 0);
+                issue(sv[i], a.v_cache, a.v_scales, row, 0);
             }
+            auto step = [&](Stage& k, Stage& v, uint64_t& v_of, Key& key) {
+                commit(k, kt, 0, v_of);
+                commit(v, vt, 0, v_of);
+                const uint64_t here = v_of;
+                const int64_t row = row_of(key, v_of);
+                key = look_up(u + 2 * kDepth * side);
+                issue(k, a.k_cache, a.k_scales, row, 0);
+                issue(v, a.v_cache, a.v_scales, row, 0);
+                asm volatile("" ::: "memory");  // (the tile is the wave's own: LDS keeps the wave's order)
+                whole_tile(kt, vt, [&](auto& s) { mask_context(s, u, here); });
+                asm volatile("" ::: "memory");
+                u += side;
+                return u < c1;
+            };
+            for (;;) {  // (written out: a loop over the stages that is left in the middle is not unrolled)
+                if (!step(sk[0], sv[0], valid[0], keys[0])) break;
+                if constexpr (kDepth > 1)
+                    if (!step(sk[1], sv[1], valid[1], keys[1])) break;
+                if constexpr (kDepth > 2)
+                    if (!step(sk[2], sv[2], valid[2], keys[2])) break;
+                static_assert(kDepth <= 3, "one step per stage");
+            }
+        }
+        for (; u < u1; u += side) {
+            const int t = u - sq.ctx_tiles;
+            fresh_rows(a.k_new, a.kn_st, a.kn_sh, t, kt, 0);
+            fresh_rows(a.v_new, a.vn_st, a.vn_sh, t, vt, 0);
             asm volatile("" ::: "memory");
-            compute<kNarrowKeys>(kt, vt, u, valid);
+            whole_tile(kt, vt, [&](auto& s) { mask_fresh(s, t); });
             asm volatile("" ::: "memory");
         }
-        // merge the four waves' states: each leaves its accumulators in its own LDS, wave d takes d block d
-        const float l = W::half_sum(w.l);
-        ml[wave * 64 + lane] = w.half ? l : w.m;
+        const float l = W::half_sum(w.l[0]);
+        if (side == 1) {
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            if (direct || has_slot(slot)) {
+#pragma unroll
+                for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, row_tile * kNarrowRows, slot, direct);
+                if (!direct) ml_slot(slot)[lane] = w.half ? l : w.m[0];
+            }
+            return;
+        }
+        // merge the states of a head's waves: each leaves its accumulators in its own LDS, and takes every side-th d block
+        ml[wave * 64 + lane] = w.half ? l : w.m[0];
         f32x4* mine = reinterpret_cast<f32x4*>(lds + wave * kAccBytes);
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-                mine[(d * 4 + x) * 64 + lane] = f32x4{w.o[d][4 * x], w.o[d][4 * x + 1], w.o[d][4 * x + 2], w.o[d][4 * x + 3]};
+                mine[(d * 4 + x) * 64 + lane] = f32x4{w.o[d][0][4 * x], w.o[d][0][4 * x + 1], w.o[d][0][4 * x + 2], w.o[d][0][4 * x + 3]};
         lds_barrier();
-        float top = -INFINITY, sum = 0.0f, f[kWgWaves];
-#pragma unroll
-        for (int i = 0; i < kWgWaves; ++i) top = fmaxf(top, ml[i * 64 + w.col]);
+        const int from = my_head << side_shift;
+        float top = -INFINITY, sum = 0.0f;
+        for (int i = from; i < from + side; ++i) top = fmaxf(top, ml[i * 64 + w.col]);
         const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < kWgWaves; ++i) {
-            f[i] = __builtin_amdgcn_exp2f(ml[i * 64 + w.col] - base);
-            sum += f[i] * ml[i * 64 + 32 + w.col];
-        }
-        if (wave < NDB) {
+        for (int i = from; i < from + side; ++i) sum += __builtin_amdgcn_exp2f(ml[i * 64 + w.col] - base) * ml[i * 64 + 32 + w.col];
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        for (int d = wave & (side - 1); d < NDB; d += side) {
             f32x16 o;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                f32x4 s = {0, 0, 0, 0};
+            for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+            for (int i = from; i < from + side; ++i) {
+                const float f = __builtin_amdgcn_exp2f(ml[i * 64 + w.col] - base);
 #pragma unroll
-                for (int i = 0; i < kWgWaves; ++i) {
-                    const f32x4 p = reinterpret_cast<const f32x4*>(lds + i * kAccBytes)[(wave * 4 + x) * 64 + lane];
-                    // (a wave without a visible key adds nothing, whatever 0 * p would be)
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 p = reinterpret_cast<const f32x4*>(lds + i * kAccBytes)[(d * 4 + x) * 64 + lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[j] += f[i] == 0.0f ? 0.0f : f[i] * p[j];
+                    for (int j = 0; j < 4; ++j) o[4 * x + j] += f * p[j];
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[4 * x + j] = s[j];
             }
-            const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-            if (direct || slot < a.n_slots) {
-                put(o, wave, inv, row_tile * kNarrowRows, slot, direct);
-                if (!direct && wave == 0) ml_slot(slot)[lane] = w.half ? sum : top;
-            }
+            if (direct || has_slot(slot)) put(o, d, inv, row_tile * kNarrowRows, slot, direct);
         }
+        if (!direct && (wave & (side - 1)) == 0 && has_slot(slot)) ml_slot(slot)[lane] = w.half ? sum : top;
         lds_barrier();
     }
 };
 
-// Inclusive scan of three values over the workgroup; returns the totals through the references' last thread.
 struct Sums {
-    int64_t cost;
-    int blocks, comb;
+    int64_t cost;      // of the launch's kind
+    int blocks, comb;  // piece slots of its items; row blocks of the merge
+    DFX_D void operator+=(const Sums& o) {
+        cost += o.cost;
+        blocks += o.blocks;
+        comb += o.comb;
+    }
 };
-DFX_D Sums scan_up(Sums v, int by) {
-    Sums r;
-    const int from = (threadIdx.x & 63) - by;
+template <bool WIDE>
+DFX_D Sums sums_of(const SplitArgs& a, const Seq& s, int v) {
+    const Costs k(a, !WIDE);
+    const int items = s.narrow != WIDE ? a.h_kv / k.heads * s.row_tiles : 0;
+    return Sums{static_cast<int64_t>(items) * item_cost(k, s.tiles), items * k.blocks, v >= a.n_groups ? a.h_kv * ((s.rows + 31) / 32) : 0};
+}
+DFX_D Sums lane_below(Sums v, int by) {
+    const int from = static_cast<int>(threadIdx.x & 63) - by;
     const int at = (from < 0 ? 0 : from) * 4;
     const int lo = __builtin_amdgcn_ds_bpermute(at, static_cast<int>(v.cost)), hi = __builtin_amdgcn_ds_bpermute(at, static_cast<int>(v.cost >> 32));
+    Sums r;
     r.cost = static_cast<int64_t>(static_cast<uint32_t>(lo)) | (static_cast<int64_t>(hi) << 32);
     r.blocks = __builtin_amdgcn_ds_bpermute(at, v.blocks);
     r.comb = __builtin_amdgcn_ds_bpermute(at, v.comb);
-    if (from < 0) r = Sums{0, 0, 0};
-    return r;
+    return from < 0 ? Sums{0, 0, 0} : r;
 }
 
-template <int HD, int KV>
-__global__ void __launch_bounds__(kWgThreads, 2) split_attn_kernel(const SplitArgs a) {
-    using T = Split<HD, KV>;
+DFX_D Seq uniform_seq(const Seq& s) {  // (what LDS returns is a vector register to the compiler)
+    return Seq{uniform(s.tok0), uniform(s.rows), uniform(s.key0), uniform(s.key1), uniform(s.new0), uniform(s.n_new), uniform(s.table),
+               uniform(s.prefix), uniform(s.seq0), uniform(s.seq1), uniform(s.tiles), uniform(s.ctx_tiles), uniform(s.row_tiles),
+               uniform(s.narrow) != 0, uniform(s.group)};
+}
+
+template <int HD, int KV, bool WIDE>
+__global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(const SplitArgs a) {
+    using T = Split<HD, KV, WIDE>;
+    constexpr int kWgWaves = Kind<WIDE>::kWaves, kWgThreads = Kind<WIDE>::kThreads;
     __shared__ __attribute__((aligned(256))) uint8_t lds[T::kLds];
     __shared__ float ml[kWgWaves * 64];
     __shared__ Sums wave_sum[kWgWaves];
     __shared__ int first_v, first_blocks;
     __shared__ int64_t first_cost;
+    __shared__ Seq first_seq;
     const int tid = threadIdx.x;
 
     // the work list: each thread a run of virtual sequences, then a scan
     const int n = a.n_groups + a.n_seqs;
     const int per = (n + kWgThreads - 1) / kWgThreads;
+    const Costs kinds(a, !WIDE);
+    const Seq my_first = seq_of(a, min(tid * per, n - 1));  // (with up to a virtual sequence per thread, read once)
+    auto seq_at = [&](int i) { return i == 0 ? my_first : seq_of(a, tid * per + i); };
     Sums mine = {0, 0, 0};
     for (int i = 0; i < per; ++i) {
         const int v = tid * per + i;
         if (v >= n) break;
-        const Seq s = seq_of(a, v);
-        const int items = a.h_kv * s.row_tiles;
-        mine.cost += static_cast<int64_t>(items) * s.tiles * s.cost();
-        mine.blocks += items * s.row_blocks();
-        if (v >= a.n_groups) mine.comb += a.h_kv * ((s.rows + 31) / 32);
+        mine += sums_of<WIDE>(a, seq_at(i), v);
     }
     Sums upto = mine;
 #pragma unroll
-    for (int by = 1; by < 64; by *= 2) {
-        const Sums o = scan_up(upto, by);
-        upto.cost += o.cost;
-        upto.blocks += o.blocks;
-        upto.comb += o.comb;
-    }
+    for (int by = 1; by < 64; by *= 2) upto += lane_below(upto, by);
     if ((tid & 63) == 63) wave_sum[tid >> 6] = upto;
     __syncthreads();
     Sums total = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < kWgWaves; ++i) {
-        if (i < (tid >> 6)) {
-            upto.cost += wave_sum[i].cost;
-            upto.blocks += wave_sum[i].blocks;
-            upto.comb += wave_sum[i].comb;
-        }
-        total.cost += wave_sum[i].cost;
-        total.blocks += wave_sum[i].blocks;
-        total.comb += wave_sum[i].comb;
+        if (i < (tid >> 6)) upto += wave_sum[i];
+        total += wave_sum[i];
     }
-    int n_wg = a.n_wg;
-    if (total.cost / kMinCost < n_wg) n_wg = static_cast<int>(max(total.cost / kMinCost, static_cast<int64_t>(1)));
-    // neighbouring ranges (the row tiles that read the same keys) on one XCD: workgroups go to the eight in turn
-    const int per_xcd = (n_wg + 7) / 8;
-    const int wg = static_cast<int>(blockIdx.x) / 8 < per_xcd ? static_cast<int>(blockIdx.x) % 8 * per_xcd + static_cast<int>(blockIdx.x) / 8 : n_wg;
-    if (blockIdx.x == 0) {  // for the merge
-        if (tid == 0) *reinterpret_cast<Header*>(a.workspace) = Header{total.cost, n_wg, total.comb};
+    int n_wg = a.n_wg[WIDE];
+    if (total.cost / kinds.least < n_wg) n_wg = static_cast<int>(max(total.cost / kinds.least, static_cast<int64_t>(1)));
+    if (blockIdx.x == 0) {  // the list, for the merge; the others work
+        if (tid == 0) reinterpret_cast<Header*>(a.workspace)[WIDE] = Header{total.cost, n_wg, total.comb};
         Sums at = {upto.cost - mine.cost, upto.blocks - mine.blocks, upto.comb - mine.comb};
+        int* comb = reinterpret_cast<int*>(a.workspace + a.comb_off);
         for (int i = 0; i < per; ++i) {
             const int v = tid * per + i;
             if (v >= n) break;
-            const Seq s = seq_of(a, v);
-            const int items = a.h_kv * s.row_tiles;
-            reinterpret_cast<TabEntry*>(a.workspace + a.tab_off)[v] = TabEntry{at.cost, at.blocks, 0};
-            if (v >= a.n_groups) reinterpret_cast<int*>(a.workspace + a.comb_off)[v - a.n_groups] = at.comb;
-            at.cost += static_cast<int64_t>(items) * s.tiles * s.cost();
-            at.blocks += items * s.row_blocks();
-            if (v >= a.n_groups) at.comb += a.h_kv * ((s.rows + 31) / 32);
+            const Seq s = seq_at(i);
+            if (s.narrow != WIDE)
+                reinterpret_cast<Rec*>(a.workspace + a.rec_off)[v] =
+                    Rec{at.cost, at.blocks, s.tok0, s.rows, s.tiles, s.row_tiles, s.prefix > 0 ? s.group : -1, s.narrow, s.key1 > 0 || s.n_new > 0};
+            if (!WIDE && v >= a.n_groups) comb[v - a.n_groups] = at.comb;
+            at += sums_of<WIDE>(a, s, v);
         }
+        if (!WIDE && tid == 0) comb[a.n_seqs] = total.comb;
+        return;
     }
+    // neighbouring ranges (the row tiles that read the same keys) on one XCD: workgroups go to the eight in turn
+    const int slot_in = static_cast<int>(blockIdx.x - 1) / 8, per_xcd = (n_wg + 7) / 8;
+    const int wg = slot_in < per_xcd ? static_cast<int>(blockIdx.x - 1) % 8 * per_xcd + slot_in : n_wg;
     if (wg >= n_wg || total.cost == 0) return;
     const int64_t c0 = range_start(wg, total.cost, n_wg), c1 = range_start(wg + 1, total.cost, n_wg);
     if (c0 >= c1) return;
     if (upto.cost > c0 && upto.cost - mine.cost <= c0) {  // this thread's run holds the first unit
-        int64_t cost = upto.cost - mine.cost;
-        int blocks = upto.blocks - mine.blocks;
+        Sums at = {upto.cost - mine.cost, upto.blocks - mine.blocks, 0};
         for (int i = 0; i < per; ++i) {
             const int v = tid * per + i;
-            const Seq s = seq_of(a, v);
-            const int items = a.h_kv * s.row_tiles;
-            const int64_t here = static_cast<int64_t>(items) * s.tiles * s.cost();
-            if (cost + here > c0) {
+            const Seq s = seq_at(i);
+            const Sums here = sums_of<WIDE>(a, s, v);
+            if (at.cost + here.cost > c0) {
                 first_v = v;
-                first_cost = cost;
-                first_blocks = blocks;
+                first_cost = at.cost;
+                first_blocks = at.blocks;
+                first_seq = s;
                 break;
             }
-            cost += here;
-            blocks += items * s.row_blocks();
+            at += here;
         }
     }
     __syncthreads();
     int64_t cost = first_cost;
-    int blocks = first_blocks;
+    cost = static_cast<int64_t>(static_cast<uint32_t>(uniform(static_cast<int>(cost)))) | (static_cast<int64_t>(uniform(static_cast<int>(cost >> 32))) << 32);
+    int blocks = uniform(first_blocks);
     T t(a, lds, ml, tid);
-    for (int v = uniform(first_v); v < n && cost < c1; ++v) {
-        t.sq = seq_of(a, v);
+    t.sq = uniform_seq(first_seq);
+    for (int v = uniform(first_v);;) {
         const Seq& s = t.sq;
-        const int items = a.h_kv * s.row_tiles, unit = s.cost();
-        const int64_t item_cost = static_cast<int64_t>(s.tiles) * unit;
-        if (item_cost > 0) {
-            int j = cost < c0 ? static_cast<int>((c0 - cost) / item_cost) : 0;
-            for (; j < items; ++j) {
-                const int64_t from = cost + j * item_cost;
-                if (from >= c1) break;
-                const int u0 = from >= c0 ? 0 : static_cast<int>((c0 - from + unit - 1) / unit);
-                const int u1 = static_cast<int>(min(static_cast<int64_t>(s.tiles), (c1 - from + unit - 1) / unit));
-                if (u0 >= u1) continue;
-                t.kvh = j / s.row_tiles;
-                t.row_tile = j - t.kvh * s.row_tiles;
-                const bool is_group = v < a.n_groups;
-                const bool direct = !is_group && s.prefix == 0 && u0 == 0 && u1 == s.tiles;
-                const int64_t slot = static_cast<int64_t>(wg) * (kWideRows / 32) + blocks + j * s.row_blocks();
-                if (s.narrow) t.narrow(u0, u1, is_group, slot, direct);
-                else t.wide(u0, u1, is_group, slot, direct);
+        if (s.narrow != WIDE) {
+            const int items = a.h_kv / kinds.heads * s.row_tiles, each = item_cost(kinds, s.tiles);
+            if (each > 0) {
+                int j = cost < c0 ? static_cast<int>((c0 - cost) / each) : 0;
+                for (; j < items; ++j) {
+                    const int64_t from = cost + static_cast<int64_t>(j) * each;
+                    if (from >= c1) break;
+                    const int u0 = from >= c0 ? 0 : static_cast<int>(c0 - from);
+                    const int u1 = static_cast<int>(min(static_cast<int64_t>(s.tiles), c1 - from));
+                    if (u0 >= u1) continue;
+                    const int head = j / s.row_tiles;  // or group of heads
+                    t.kvh = head;
+                    t.row_tile = j - head * s.row_tiles;
+                    const bool is_group = v < a.n_groups;
+                    const bool direct = !is_group && s.prefix == 0 && u0 == 0 && u1 == s.tiles;
+                    const int64_t slot = a.first_slot[WIDE] + (static_cast<int64_t>(wg) + j) * kinds.blocks + blocks;
+                    if constexpr (WIDE) t.wide(u0, u1, is_group, slot, direct);
+                    else t.narrow(u0, u1, is_group, slot, direct);
+                }
             }
+            cost += static_cast<int64_t>(items) * each;
+            blocks += items * kinds.blocks;
         }
-        cost += items * item_cost;
-        blocks += items * s.row_blocks();
+        if (++v >= n || cost >= c1) break;
+        t.sq = seq_of(a, v);
     }
 }
 
 // ---- merge -------------------------------------------------------------------------------------
-// One workgroup per (sequence, KV head, 32 rows); wave d merges d block d (head_dim 64: two waves per d block, every
-// second piece each).
-template <int HD>
-__global__ void __launch_bounds__(kWgThreads) split_merge_kernel(const SplitArgs a) {
-    constexpr int NDB = HD / 32, kShare = kWgWaves / NDB;
+// One workgroup per (sequence, KV head, 32 rows): NDB waves for the d blocks, times kShare that take every kShare-th piece of the row,
+// kAtOnce of them together.  Bound by latency: the list and the pieces lie in memory that another XCD wrote, so everything that may be
+// needed of the list is asked for at once.  (The order of the sums is the pieces', whoever finished first.)
+constexpr int kAtOnce = 4;
+// Few row blocks have many pieces each (the work is spread over all workgroups), many have few.
+constexpr int kMergeWavesFew = 16, kMergeWavesMany = 4, kFewBlocks = 1024;
+
+template <int HD, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) split_merge_kernel(const SplitArgs a) {
+    constexpr int NDB = HD / 32, kShare = WAVES / NDB;
     constexpr int kAccBytes = 32 * HD * 4;
-    __shared__ int found;
-    __shared__ float part[kWgWaves][18][64];
+    __shared__ int found_at;
+    __shared__ Rec found_rec, group_rec;
+    __shared__ float part[kShare > 1 ? WAVES : 1][18][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, half = lane >> 5;
-    const Header h = *reinterpret_cast<const Header*>(a.workspace);
+    const Header* heads = reinterpret_cast<const Header*>(a.workspace);
     const int x = blockIdx.x;
-    if (x >= h.n_comb) return;
     const int* comb = reinterpret_cast<const int*>(a.workspace + a.comb_off);
-    for (int s = tid; s < a.n_seqs; s += kWgThreads) {
-        const int next = s + 1 < a.n_seqs ? comb[s + 1] : h.n_comb;
-        if (comb[s] <= x && x < next) found = s;
+    const Rec* recs = reinterpret_cast<const Rec*>(a.workspace + a.rec_off);
+    const Header head_of[2] = {heads[0], heads[1]};
+    const Rec my_group = recs[min(tid, a.n_groups)];
+    for (int s = tid; s < a.n_seqs; s += WAVES * 64) {
+        const int from = comb[s], to = comb[s + 1];
+        const Rec r = recs[a.n_groups + s];
+        if (from <= x && x < to) {
+            found_at = from;
+            found_rec = r;
+        }
     }
+    if (x >= head_of[0].n_comb) return;
     __syncthreads();
-    const int s = uniform(found), v = a.n_groups + s;
-    const Seq q = seq_of(a, v);
-    if (q.key1 == 0 && q.n_new == 0) return;  // no key at all: the rows stay as they are
+    const Rec q = found_rec;
+    if (!q.has_keys) return;  // no key at all: the rows stay as they are
     const int rbs = (q.rows + 31) / 32;
-    const int local = x - comb[s], kvh = local / rbs, rb = local - kvh * rbs;
-    const TabEntry* tab = reinterpret_cast<const TabEntry*>(a.workspace + a.tab_off);
+    const int local = x - found_at, kvh = local / rbs, rb = local - kvh * rbs;
     const int row = rb * 32 + col;
     const bool live = row < q.rows;
 
-    // the pieces of this lane's row: own item, then the group's
-    int w0[2] = {0, 0}, n[2] = {0, 0}, at_col[2] = {col, 0};
-    int64_t slot0[2] = {0, 0};
+    // the pieces of this lane's row: its own item's, then its group's.  slot of piece i: first + i * step
+    int64_t first[2] = {0, 0};
+    int n[2] = {0, 0}, at_col[2] = {col, 0}, step[2] = {1, 1};
+    auto pieces = [&](const Rec& r, int k, int at_row) {
+        const Header h = r.narrow ? head_of[0] : head_of[1];
+        const Costs c(a, r.narrow);
+        const int most = r.narrow ? kNarrowRows : kWideRows, t = at_row / most;
+        const int64_t j = static_cast<int64_t>(kvh / c.heads) * r.row_tiles + t, from = r.cost + j * item_cost(c, r.tiles);
+        const int w0 = owner_of(from, h.total, h.n_wg);
+        n[k] = owner_of(from + r.tiles - 1, h.total, h.n_wg) - w0 + 1;
+        first[k] = a.first_slot[r.narrow ? 0 : 1] + (w0 + j) * c.blocks + r.blocks + (r.narrow ? kvh % c.heads : (at_row - t * most) / 32);
+        step[k] = c.blocks;
+        at_col[k] = at_row & 31;
+    };
     if (q.tiles > 0) {
-        const int t = q.narrow ? rb : rb / 4;
-        const int64_t j = static_cast<int64_t>(kvh) * q.row_tiles + t, unit = q.cost();
-        const int64_t from = tab[v].cost + j * q.tiles * unit;
-        w0[0] = owner_of(from, h.total, h.n_wg);
-        n[0] = owner_of(from + (q.tiles - 1) * unit, h.total, h.n_wg) - w0[0] + 1;
-        slot0[0] = tab[v].blocks + j * q.row_blocks() + (q.narrow ? 0 : rb & 3);
-        if (q.prefix == 0 && n[0] == 1) return;  // written by its only workgroup
+        pieces(q, 0, rb * 32);
+        at_col[0] = col;
+        if (q.group < 0 && n[0] == 1) return;  // written by its only workgroup
     }
-    if (q.prefix > 0) {
-        int lo = 0, hi = a.n_groups;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.group_cu[mid] <= s) lo = mid;
-            else hi = mid;
+    if (q.group >= 0) {
+        if (a.n_groups < WAVES * 64) {
+            if (tid == q.group) group_rec = my_group;
+        } else if (tid == 0) {
+            group_rec = recs[q.group];
         }
-        const Seq g = seq_of(a, lo);
-        if (g.tiles > 0) {
-            const int grow = (q.tok0 - g.tok0) * a.group_heads + row;
-            const int rt = g.narrow ? kNarrowRows : kWideRows, t = grow / rt;
-            const int64_t j = static_cast<int64_t>(kvh) * g.row_tiles + t, unit = g.cost();
-            const int64_t from = tab[lo].cost + j * g.tiles * unit;
-            w0[1] = owner_of(from, h.total, h.n_wg);
-            n[1] = live ? owner_of(from + (g.tiles - 1) * unit, h.total, h.n_wg) - w0[1] + 1 : 0;
-            slot0[1] = tab[lo].blocks + j * g.row_blocks() + (grow - t * rt) / 32;
-            at_col[1] = grow & 31;
-        }
+        __syncthreads();
+        const Rec g = group_rec;
+        if (g.tiles > 0) pieces(g, 1, max(0, (q.tok0 - g.tok0) * a.group_heads + (live ? row : 0)));
     }
     const int d = wave % NDB, share = wave / NDB;
     float m = -INFINITY, l = 0.0f;
     f32x4 o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = f32x4{0, 0, 0, 0};
+    const int all = live ? n[0] + n[1] : 0;
+    const int64_t slots = a.first_slot[1] + a.n_slots[1];
+    for (int i0 = share; __builtin_amdgcn_ballot_w64(i0 < all) != 0; i0 += kShare * kAtOnce) {
+        float pm[kAtOnce], pl[kAtOnce];
+        f32x4 po[kAtOnce][4];
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-        const int c = at_col[kind];
-        for (int i = share; __builtin_amdgcn_ballot_w64(i < n[kind]) != 0; i += kShare) {
-            const int64_t slot = slot0[kind] + static_cast<int64_t>(w0[kind] + i) * (kWideRows / 32);
-            if (!live || i >= n[kind] || slot >= a.n_slots) continue;
-            const float* ml = reinterpret_cast<const float*>(a.workspace + a.ml_off) + slot * 64;
-            const f32x4* acc = reinterpret_cast<const f32x4*>(a.workspace + a.slot_off + slot * kAccBytes);
-            const float pm = ml[c], pl = ml[32 + c];
-            f32x4 po[4];
+        for (int y = 0; y < kAtOnce; ++y) {
+            const int i = i0 + y * kShare;
+            const bool mine = i < n[0];
+            const int64_t slot = mine ? first[0] + static_cast<int64_t>(i) * step[0] : first[1] + static_cast<int64_t>(i - n[0]) * step[1];
+            const int c = mine ? at_col[0] : at_col[1];
+            const bool is = i < all && slot >= 0 && slot < slots;
+            const float* ml = reinterpret_cast<const float*>(a.workspace + a.ml_off) + (is ? slot : 0) * 64;
+            const f32x4* acc = reinterpret_cast<const f32x4*>(a.workspace + a.slot_off + (is ? slot : 0) * kAccBytes);
+            pm[y] = -INFINITY;
+            pl[y] = 0.0f;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) po[y] = acc[(d * 4 + y) * 64 + half * 32 + c];
-            if (pm == -INFINITY && pl == 0.0f) continue;  // no visible key in the piece
-            const float next = fmaxf(m, pm);
-            const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next), add = __builtin_amdgcn_exp2f(pm - next);
-            m = next;
-            l = l * keep + pl * add;
+            for (int z = 0; z < 4; ++z) po[y][z] = f32x4{0, 0, 0, 0};
+            if (is) {
+                pm[y] = ml[c];
+                pl[y] = ml[32 + c];
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+                for (int z = 0; z < 4; ++z) po[y][z] = acc[(d * 4 + z) * 64 + half * 32 + c];
+            }
+        }
+        float top = m;
 #pragma unroll
-                for (int z = 0; z < 4; ++z) o[y][z] = o[y][z] * keep + po[y][z] * add;
+        for (int y = 0; y < kAtOnce; ++y) top = fmaxf(top, pm[y]);
+        const float base = top == -INFINITY ? 0.0f : top;  // (pieces without a visible key: weight 2^-inf = 0 of zeros)
+        const float keep = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) o[z] *= keep;
+#pragma unroll
+        for (int y = 0; y < kAtOnce; ++y) {
+            const float f = __builtin_amdgcn_exp2f(pm[y] - base);
+            l += pl[y] * f;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) o[z] += po[y][z] * f;
         }
     }
     if constexpr (kShare > 1) {
@@ -816,13 +1108,17 @@ __global__ void __launch_bounds__(kWgThreads) split_merge_kernel(const SplitArgs
         }
         __syncthreads();
         if (share > 0) return;
-        const int other = wave + NDB;
-        const float pm = part[other][0][lane], pl = part[other][1][lane];
-        const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.0f : next;
-        const float keep = __builtin_amdgcn_exp2f(m - base), add = __builtin_amdgcn_exp2f(pm - base);
-        l = l * keep + pl * add;
 #pragma unroll
-        for (int y = 0; y < 16; ++y) o[y >> 2][y & 3] = o[y >> 2][y & 3] * keep + part[other][2 + y][lane] * add;
+        for (int i = 1; i < kShare; ++i) {
+            const int other = wave + i * NDB;
+            const float pm = part[other][0][lane], pl = part[other][1][lane];
+            const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
+            const float keep = __builtin_amdgcn_exp2f(m - base), add = __builtin_amdgcn_exp2f(pm - base);
+            m = top;
+            l = l * keep + pl * add;
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y >> 2][y & 3] = o[y >> 2][y & 3] * keep + part[other][2 + y][lane] * add;
+        }
     }
     if (!live) return;
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -851,38 +1147,51 @@ int compute_units() {
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Sizes of the launch and of its workspace; a status.
+// Sizes of the launches and of their workspace; a status.
 int lay_out(const dfx_split_attn_params* p, SplitArgs& a, int64_t& comb_blocks, int64_t& bytes) {
     if (!p || p->num_seqs < 0 || p->num_groups < 0 || p->num_q_heads <= 0 || p->num_kv_heads <= 0 || p->num_q_tokens < 0 ||
-        p->num_new_tokens < 0 || p->max_workgroups < 0)
+        p->num_new_tokens < 0 || p->max_workgroups < 0 || p->max_seqlen_q < 0)
         return DFX_ERR_INVALID_ARG;
     if (p->num_q_heads % p->num_kv_heads != 0) return DFX_ERR_INVALID_ARG;
     if (p->head_dim != 64 && p->head_dim != 128) return DFX_ERR_UNSUPPORTED;
     if (p->num_seqs > 65535 || p->num_groups > p->num_seqs + 1 || p->num_q_tokens > INT32_MAX / p->num_q_heads ||
         p->num_new_tokens > INT32_MAX || p->max_workgroups > 65535)
         return DFX_ERR_UNSUPPORTED;
-    int n_wg = p->max_workgroups;
-    if (n_wg == 0) {
+    a.n_wg[0] = a.n_wg[1] = p->max_workgroups;
+    if (p->max_workgroups == 0) {  // what the device holds at once, the list's workgroup included
         const int cus = compute_units();
         if (cus < 0) return DFX_ERR_LAUNCH;
-        n_wg = 2 * cus;
+        a.n_wg[0] = 2 * cus - 1;
+        a.n_wg[1] = cus - 1 > 0 ? cus - 1 : 1;
     }
-    a.n_wg = n_wg;
     a.n_seqs = p->num_seqs;
     a.n_groups = p->num_groups;
     a.h_kv = p->num_kv_heads;
     a.group_heads = p->num_q_heads / p->num_kv_heads;
-    const int64_t rows32 = (p->num_q_tokens * a.group_heads + 31) / 32;
+    // rows of the largest virtual sequence, as far as the host knows: without wide items there is no wide launch
+    const int64_t rows = p->num_q_tokens * a.group_heads;
+    int64_t most = p->max_seqlen_q > 0 ? static_cast<int64_t>(p->max_seqlen_q) * a.group_heads : rows;
+    if (most > rows || p->num_groups > 0) most = rows;
+    a.use_wide = most > kNarrowMost;
+    const int64_t rows32 = (rows + 31) / 32, vs = static_cast<int64_t>(p->num_seqs) + p->num_groups;
     comb_blocks = a.h_kv * (rows32 + p->num_seqs);
-    // (an item of R rows takes at most R / 32 + 4 blocks)
-    const int64_t blocks = a.h_kv * ((p->num_groups > 0 ? 2 : 1) * rows32 + 4 * (static_cast<int64_t>(p->num_seqs) + p->num_groups));
-    a.n_slots = static_cast<int64_t>(n_wg) * (kWideRows / 32) + blocks;
-    if (comb_blocks > UINT32_MAX / kWgThreads || blocks > INT32_MAX) return DFX_ERR_UNSUPPORTED;
-    a.tab_off = 256;
-    a.comb_off = a.tab_off + round_up((static_cast<int64_t>(p->num_seqs) + p->num_groups) * static_cast<int64_t>(sizeof(TabEntry)), 256);
-    a.ml_off = a.comb_off + round_up(static_cast<int64_t>(p->num_seqs) * 4, 256);
-    a.slot_off = a.ml_off + a.n_slots * 256;
-    bytes = a.slot_off + a.n_slots * 32 * p->head_dim * 4;
+    // (an item of R rows takes at most R / 32 + 1 slots if it is narrow, R / 32 + 8 if it is wide, which needs more than kNarrowMost rows)
+    const int64_t copies = (p->num_groups > 0 ? 2 : 1) * rows32;
+    const int64_t wide_vs = vs < copies * 32 / kNarrowMost ? vs : copies * 32 / kNarrowMost;
+    // (and chunks of at least a workgroup's share add at most an item per workgroup; a piece's slot is its workgroup's and its item's index)
+    a.heads_shift = a.h_kv % 4 == 0 ? 2 : a.h_kv % 2 == 0 ? 1 : 0;
+    // (a piece's slot is the sum of its workgroup's and its item's index)
+    a.n_slots[0] = (static_cast<int64_t>(a.n_wg[0]) << a.heads_shift) + a.h_kv * (copies + vs);
+    a.n_slots[1] = a.use_wide ? (a.n_wg[1] + a.h_kv * wide_vs) * (kWideRows / 32) + a.h_kv * copies : 0;
+    a.first_slot[0] = 0;
+    a.first_slot[1] = a.n_slots[0];
+    const int64_t slots = a.n_slots[0] + a.n_slots[1];
+    if (comb_blocks > UINT32_MAX / (kMergeWavesFew * 64) || slots > INT32_MAX) return DFX_ERR_UNSUPPORTED;
+    a.rec_off = 256;
+    a.comb_off = a.rec_off + round_up(vs * static_cast<int64_t>(sizeof(Rec)), 256);
+    a.ml_off = a.comb_off + round_up((static_cast<int64_t>(p->num_seqs) + 1) * 4, 256);
+    a.slot_off = a.ml_off + slots * 256;
+    bytes = a.slot_off + slots * 32 * p->head_dim * 4;
     return DFX_OK;
 }
 
@@ -919,25 +1228,30 @@ extern "C" int dfx_split_attn(const dfx_split_attn_params* p, dfx_stream_t strea
                                p->o_stride_token, p->o_stride_head};
     for (int64_t s : strides)
         if (s % 8 || s < 0) return DFX_ERR_INVALID_ARG;
-    if (p->k_cache) {
+    const bool cached = p->k_cache && p->n_pages != 0 && p->max_pages_per_seq != 0;
+    if (cached) {
         if (!p->v_cache || !p->block_tables || !p->context_lens || p->page_size <= 0 || p->n_pages < 0 || p->max_pages_per_seq < 0 ||
             p->block_table_stride < 0)
             return DFX_ERR_INVALID_ARG;
         if (mx != (p->k_scales != nullptr) || mx != (p->v_scales != nullptr)) return DFX_ERR_INVALID_ARG;
         if (p->n_pages > INT32_MAX) return DFX_ERR_UNSUPPORTED;
-        const int64_t row = mx ? mx_row_bytes(p->kv_dtype == DFX_KV_MX_E2M1, p->head_dim) : 0;
+        int64_t page_bytes, token_bytes, head_bytes;
         if (mx) {
-            a.c_sh = row;
-            a.c_st = row * p->num_kv_heads;
-            a.c_sp = a.c_st * p->page_size;
+            head_bytes = mx_row_bytes(p->kv_dtype == DFX_KV_MX_E2M1, p->head_dim);
+            token_bytes = head_bytes * p->num_kv_heads;
+            page_bytes = token_bytes * p->page_size;
         } else {
             if (p->cache_stride_page % 8 || p->cache_stride_token % 8 || p->cache_stride_head % 8 || p->cache_stride_page < 0 ||
                 p->cache_stride_token < 0 || p->cache_stride_head < 0)
                 return DFX_ERR_INVALID_ARG;
-            a.c_sp = p->cache_stride_page * 2;
-            a.c_st = p->cache_stride_token * 2;
-            a.c_sh = p->cache_stride_head * 2;
+            page_bytes = p->cache_stride_page * 2;
+            token_bytes = p->cache_stride_token * 2;
+            head_bytes = p->cache_stride_head * 2;
         }
+        if (page_bytes > UINT32_MAX || token_bytes > UINT32_MAX || head_bytes > UINT32_MAX) return DFX_ERR_UNSUPPORTED;
+        a.c_sp = static_cast<uint32_t>(page_bytes);
+        a.c_st = static_cast<uint32_t>(token_bytes);
+        a.c_sh = static_cast<uint32_t>(head_bytes);
         a.block_tables = p->block_tables;
         a.context_lens = p->context_lens;
         a.bt_stride = p->block_table_stride;
@@ -946,7 +1260,11 @@ extern "C" int dfx_split_attn(const dfx_split_attn_params* p, dfx_stream_t strea
         a.page_size = p->page_size;
         a.page_shift = (p->page_size & (p->page_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(p->page_size)) : -1;
     } else {
-        a.page_size = 1;
+        // No cache: no context and no prefix.  The kernel's loads are not conditional -- a key without a cache row loads the first row of
+        // the cache and drops it, a tile behind the last its table row's last entry --, they read the workspace here.
+        a.page_size = a.max_pages = 1;
+        a.block_tables = static_cast<const int32_t*>(p->workspace);
+        a.n_groups = 0;
     }
     if (!p->workspace || p->workspace_bytes < bytes) return DFX_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(p->workspace) % 256) return DFX_ERR_INVALID_ARG;
@@ -954,8 +1272,8 @@ extern "C" int dfx_split_attn(const dfx_split_attn_params* p, dfx_stream_t strea
     a.k_new = static_cast<const uint16_t*>(p->k_new);
     a.v_new = static_cast<const uint16_t*>(p->v_new);
     a.out = static_cast<uint16_t*>(p->out);
-    a.k_cache = static_cast<const uint8_t*>(p->k_cache);
-    a.v_cache = static_cast<const uint8_t*>(p->v_cache);
+    a.k_cache = static_cast<const uint8_t*>(cached ? p->k_cache : p->workspace);
+    a.v_cache = static_cast<const uint8_t*>(cached ? p->v_cache : p->workspace);
     a.k_scales = static_cast<const uint8_t*>(p->k_scales);
     a.v_scales = static_cast<const uint8_t*>(p->v_scales);
     a.cu_q = p->cu_seqlens_q;
@@ -977,17 +1295,26 @@ extern "C" int dfx_split_attn(const dfx_split_attn_params* p, dfx_stream_t strea
     a.block_causal = p->mask_mode == DFX_MASK_BLOCK_CAUSAL;
     a.c = p->scale * 1.4426950408889634f;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(a.n_wg)), block(kWgThreads), merge(static_cast<unsigned>(comb));
-    const int kv = !a.k_cache || !mx ? kBf16 : p->kv_dtype == DFX_KV_MX_E4M3 ? kMx8 : kMx4;
+    const int kv = !cached || !mx ? kBf16 : p->kv_dtype == DFX_KV_MX_E4M3 ? kMx8 : kMx4;
+#define DFX_SPLIT_KIND(HD_, WIDE_)                                                                          \
+    do {                                                                                                    \
+        auto kern = kv == kBf16  ? split_attn_kernel<HD_, kBf16, WIDE_>                                     \
+                    : kv == kMx8 ? split_attn_kernel<HD_, kMx8, WIDE_>                                      \
+                                 : split_attn_kernel<HD_, kMx4, WIDE_>;                                     \
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(a.n_wg[WIDE_]) + 1), dim3(Kind<WIDE_>::kThreads), 0, st, a);          \
+    } while (0)
 #define DFX_SPLIT(HD_)                                                                                      \
     do {                                                                                                    \
-        auto kern = kv == kBf16 ? split_attn_kernel<HD_, kBf16>                                             \
-                                : kv == kMx8 ? split_attn_kernel<HD_, kMx8> : split_attn_kernel<HD_, kMx4>; \
-        hipLaunchKernelGGL(kern, grid, block, 0, st, a);                                                    \
-        hipLaunchKernelGGL((split_merge_kernel<HD_>), merge, block, 0, st, a);                              \
+        if (a.use_wide) DFX_SPLIT_KIND(HD_, true);                                                          \
+        DFX_SPLIT_KIND(HD_, false);                                                                         \
+        if (comb <= kFewBlocks)                                                                             \
+            hipLaunchKernelGGL((split_merge_kernel<HD_, kMergeWavesFew>), dim3(static_cast<unsigned>(comb)), dim3(kMergeWavesFew * 64), 0, st, a); \
+        else                                                                                                \
+            hipLaunchKernelGGL((split_merge_kernel<HD_, kMergeWavesMany>), dim3(static_cast<unsigned>(comb)), dim3(kMergeWavesMany * 64), 0, st, a); \
     } while (0)
     if (p->head_dim == 128) DFX_SPLIT(128);
     else DFX_SPLIT(64);
 #undef DFX_SPLIT
+#undef DFX_SPLIT_KIND
     return launch_status();
 }

@@ -401,7 +401,8 @@ void kv_load_mx(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_sc
 }
 
 // ---- split attention: microscaled caches, shared prefixes ----------------------------------------
-int64_t split_attention_workspace_bytes(const Tensor& q, int64_t num_kv_heads, int64_t num_seqs, int64_t num_groups, int64_t max_wg) {
+int64_t split_attention_workspace_bytes(const Tensor& q, int64_t num_kv_heads, int64_t num_seqs, int64_t num_groups, int64_t max_wg,
+                                        int64_t max_seqlen_q) {
     const c10::DeviceGuard guard(q.device());
     dfx_split_attn_params p = {};
     p.num_q_tokens = q.size(0);
@@ -411,6 +412,7 @@ int64_t split_attention_workspace_bytes(const Tensor& q, int64_t num_kv_heads, i
     p.num_seqs = static_cast<int32_t>(num_seqs);
     p.num_groups = static_cast<int32_t>(num_groups);
     p.max_workgroups = static_cast<int32_t>(max_wg);
+    p.max_seqlen_q = static_cast<int32_t>(max_seqlen_q);
     const int64_t n = dfx_split_attn_workspace_bytes(&p);
     if (n < 0) check(static_cast<int>(n), "dfx_split_attn_workspace_bytes");
     return n;
@@ -419,7 +421,8 @@ int64_t split_attention_workspace_bytes(const Tensor& q, int64_t num_kv_heads, i
 void split_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& k_cache, const OptTensor& v_cache,
                      const OptTensor& k_scale, const OptTensor& v_scale, Tensor out, const OptTensor& block_tables,
                      const OptTensor& context_lens, const Tensor& cu_q, const Tensor& cu_new, const OptTensor& prefix_cu_seqs,
-                     const OptTensor& prefix_lens, Tensor workspace, double scale, int64_t mask_mode, int64_t dbs, int64_t max_wg) {
+                     const OptTensor& prefix_lens, Tensor workspace, double scale, int64_t mask_mode, int64_t dbs, int64_t max_wg,
+                     int64_t max_seqlen_q) {
     const c10::DeviceGuard guard(q.device());
     TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16,
                 "q, k and v must be bf16 device tensors");
@@ -509,6 +512,7 @@ void split_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Op
     p.diffusion_block_size = static_cast<int32_t>(dbs);
     p.mask_mode = static_cast<int32_t>(mask_mode);
     p.max_workgroups = static_cast<int32_t>(max_wg);
+    p.max_seqlen_q = static_cast<int32_t>(max_seqlen_q);
     p.scale = static_cast<float>(scale);
     check(dfx_split_attn(&p, current_stream()), "dfx_split_attn");
 }
@@ -696,8 +700,9 @@ TORCH_LIBRARY(diffulex_amd, m) {
     m.def("split_attention(Tensor q, Tensor k, Tensor v, Tensor? k_cache, Tensor? v_cache, Tensor? k_scale, Tensor? v_scale, "
           "Tensor(a!) out, Tensor? block_tables, Tensor? context_lens, Tensor cu_seqlens_q, Tensor cu_seqlens_new, "
           "Tensor? prefix_cu_seqs, Tensor? prefix_lens, Tensor(b!) workspace, float scale, int mask_mode, int diffusion_block_size, "
-          "int max_workgroups) -> ()");
-    m.def("split_attention_workspace_bytes(Tensor q, int num_kv_heads, int num_seqs, int num_groups, int max_workgroups) -> int");
+          "int max_workgroups, int max_seqlen_q) -> ()");
+    m.def("split_attention_workspace_bytes(Tensor q, int num_kv_heads, int num_seqs, int num_groups, int max_workgroups, "
+          "int max_seqlen_q) -> int");
     m.def("kv_store_mx(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
           "Tensor slot_mapping) -> ()");
     m.def("kv_load_mx(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor k_new, Tensor v_new, "

@@ -98,7 +98,8 @@ def paged_attention(q, k, v, k_cache, v_cache, scale, *, block_tables, context_l
             raise _lib.DfxError("dfx_split_attn: microscaled caches and shared prefixes take the unified layout, without rope and "
                                 "static_scratch (unsupported shape)")
         out = _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_lens, cu_seqlens_q, cu_seqlens_new,
-                               mask_mode, diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens)
+                               mask_mode, diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens,
+                               max_seqlen_q)
         if store_slot_mapping is not None:
             store_kvcache_unified_layout(k, v, k_cache, v_cache, store_slot_mapping, None, k_scale, v_scale)
         return out
@@ -170,7 +171,7 @@ _split_need = {}   # launch shape -> dfx_split_attn_workspace_bytes
 
 
 def _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_lens, cu_seqlens_q, cu_seqlens_new, mask_mode,
-                     diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens):
+                     diffusion_block_size, k_scale, v_scale, max_workgroups, out, prefix_cu_seqs, prefix_lens, max_seqlen_q):
     """``dfx_split_attn``.  Its workspace needs no particular contents, so each call takes one from PyTorch's allocator (which
     orders its reuse on the stream, and gives a captured graph memory of its own)."""
     ops = _lib.ops()
@@ -180,14 +181,15 @@ def _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_len
         k_cache = v_cache = None
     num_seqs = cu_seqlens_q.numel() - 1
     groups = prefix_lens.numel() if prefix_lens is not None else 0
-    key = (q.device.index, q.shape, k.shape[1], num_seqs, groups, max_workgroups)
+    key = (q.device.index, q.shape, k.shape[1], num_seqs, groups, max_workgroups, max_seqlen_q)
     need = _split_need.get(key)
     if need is None:
-        need = _split_need[key] = int(_call(ops.split_attention_workspace_bytes, q, k.shape[1], num_seqs, groups, int(max_workgroups)))
+        need = _split_need[key] = int(_call(ops.split_attention_workspace_bytes, q, k.shape[1], num_seqs, groups, int(max_workgroups),
+                                                int(max_seqlen_q)))
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     _call(ops.split_attention, q, k, v, k_cache, v_cache, k_scale, v_scale, out, block_tables, context_lens, cu_seqlens_q,
           cu_seqlens_new, prefix_cu_seqs, prefix_lens, workspace, float(scale), int(mask_mode), int(diffusion_block_size),
-          int(max_workgroups))
+          int(max_workgroups), int(max_seqlen_q))
     return out
 
 
@@ -320,7 +322,7 @@ def dllm_flash_attn_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
         return paged_attention(
             q, k, v, k_cache, v_cache, scale, block_tables=attn_metadata.block_tables,
             context_lens=attn_metadata.context_lens, cu_seqlens_q=attn_metadata.cu_seqlens_q, cu_seqlens_new=cu_new,
-            max_seqlen_q=0, mask_mode=mask, diffusion_block_size=attn_metadata.diffusion_block_size, k_scale=k_scale,
+            max_seqlen_q=int(getattr(attn_metadata, "max_seqlen_q", 0) or 0), mask_mode=mask, diffusion_block_size=attn_metadata.diffusion_block_size, k_scale=k_scale,
             v_scale=v_scale, store_slot_mapping=store_slot_mapping, cache_layout=kv_cache_layout, rope=rope,
             prefix_cu_seqs=getattr(attn_metadata, "prefix_cu_seqs", None), prefix_lens=prefix_lens)
     if kv_cache_layout == "distinct":

@@ -527,7 +527,7 @@ int dfx_rope_kv_store(const dfx_rope_params* params, dfx_stream_t stream);
  * prefix_lens[g] / page_size are not read.  A sequence whose context is shorter than its group's prefix sees its context_lens keys
  * of it.
  *
- * Two launches (pieces, merge), planned on the device from the lengths: nothing is read back, both may be recorded into a
+ * Two or three launches (pieces, merge), planned on the device from the lengths: nothing is read back, both may be recorded into a
  * graph whose replays find other lengths, and the results do not depend on timing (pieces are merged in order).  The workspace
  * (dfx_split_attn_workspace_bytes(), 256-byte aligned, any contents) must not be shared by calls that overlap in time.
  *
@@ -565,11 +565,12 @@ typedef struct dfx_split_attn_params {
     int32_t diffusion_block_size;
     int32_t kv_dtype;       /* dfx_kv_dtype */
     int32_t mask_mode;      /* dfx_mask_mode */
-    int32_t max_workgroups; /* 0: two per compute unit */
+    int32_t max_workgroups; /* 0: as many as the device holds at once */
+    int32_t max_seqlen_q;   /* upper bound of any sequence's query rows, 0: unknown (one launch may then find nothing to do) */
     float scale;
 } dfx_split_attn_params;
 
-/* Negative: dfx_status.  Depends on num_seqs, num_groups, num_q_tokens, the head counts, head_dim and max_workgroups. */
+/* Negative: dfx_status.  Depends on num_seqs, num_groups, num_q_tokens, the head counts, head_dim, max_workgroups and max_seqlen_q. */
 int64_t dfx_split_attn_workspace_bytes(const dfx_split_attn_params* params);
 int dfx_split_attn(const dfx_split_attn_params* params, dfx_stream_t stream);
 
