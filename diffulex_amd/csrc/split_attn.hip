@@ -358,9 +358,8 @@ struct Wave {
     // the second until the first is through the pipeline), or all loads first, which does not fit the registers.
     static constexpr int kAheadK = 2;  // slabs
     static constexpr int kAheadV = 3;  // 16 keys x 32 elements each
-    //   weights of s, scores of the next tile, and the first operands of the second half
-    DFX_D void weights_and_scores(const f32x16 (&s)[2][NB], float c, bf16x8 (&p)[NB][2][2], uint32_t kt, f32x16 (&next)[2][NB], uint32_t vt,
-                                  bf16x8 (&v)[kAheadV + 1]) {
+    //   weights of s, scores of the next tile
+    DFX_D void weights_and_scores(const f32x16 (&s)[2][NB], float c, bf16x8 (&p)[NB][2][2], uint32_t kt, f32x16 (&next)[2][NB]) {
         static_assert(NB == 1, "the weights of a slab's step are those of one row block");
         constexpr int kEach = 32 / NSLAB;  // weights per step
         clear(next);
@@ -378,14 +377,9 @@ struct Wave {
             if (sl + kAheadK < NSLAB) {
                 k[(sl + kAheadK) % (kAheadK + 1)][0] = read_k(kt, 0, sl + kAheadK);
                 k[(sl + kAheadK) % (kAheadK + 1)][1] = read_k(kt, 1, sl + kAheadK);
-            } else {
-#pragma unroll
-                for (int i = (sl + kAheadK - NSLAB) * kAheadV / kAheadK; i < (sl + kAheadK - NSLAB + 1) * kAheadV / kAheadK; ++i)
-                    v[i] = read_v(vt, i / (2 * NDB), (i / NDB) & 1, i % NDB);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                next[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[sl % (kAheadK + 1)][i], q[0][sl], next[i][0], 0, 0, 0);
 #pragma unroll
                 for (int j = 0; j < kEach / 2; j += 2) {
                     const int e = sl * kEach + i * (kEach / 2) + j, t = e >> 4;
@@ -396,6 +390,8 @@ struct Wave {
                     // (wanted here: otherwise they are all made behind the last matrix instruction)
                     asm volatile("" : "+v"(w[t][(e & 15) >> 1]), "+v"(sum));
                 }
+                next[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[sl % (kAheadK + 1)][i], q[0][sl], next[i][0], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -407,11 +403,13 @@ struct Wave {
                 p[0][t][x] = __builtin_bit_cast(bf16x8, u32x4{w[t][4 * x], w[t][4 * x + 1], w[t][4 * x + 2], w[t][4 * x + 3]});
     }
     //   outputs of a tile and the largest of the next tile's scores (this half's, unscaled)
-    DFX_D void accumulate_and_top(uint32_t vt, const bf16x8 (&p)[NB][2][2], const f32x16 (&next)[2][NB], float (&top)[NB],
-                                  bf16x8 (&v)[kAheadV + 1]) {
+    DFX_D void accumulate_and_top(uint32_t vt, const bf16x8 (&p)[NB][2][2], const f32x16 (&next)[2][NB], float (&top)[NB]) {
+        bf16x8 v[kAheadV + 1];
         constexpr int kSteps = 4 * NDB;
         constexpr int kEach = 32 / kSteps;  // scores per step
         top[0] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kAheadV; ++i) v[i] = read_v(vt, i / (2 * NDB), (i / NDB) & 1, i % NDB);
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
             const int t = st / (2 * NDB), x = (st / NDB) & 1, d = st % NDB, n = st + kAheadV;
@@ -440,7 +438,7 @@ struct Split {
     static constexpr int KT = WIDE ? kWideKeys : kNarrowKeys;
     static constexpr int ROWS = WIDE ? kWideKeys / kWgWaves : kNarrowKeys;             // rows of a tile that one wave moves
     static constexpr int kMat = KT * L::ROWB;                                          // K or V of a tile in LDS
-    static constexpr int kLds = WIDE ? 4 * kMat : kWgWaves * 2 * kMat;                 // two buffers each; a tile per wave
+    static constexpr int kLds = WIDE ? 6 * kMat : kWgWaves * 2 * kMat;                 // three buffers each; a tile per wave
     static constexpr int kAccBytes = 32 * HD * 4;
     static constexpr int kPer = 64 / kChunks;                                          // rows per load of the wave
     static constexpr int kLoads = ROWS > kPer ? ROWS / kPer : 1;                       // (one that some lanes only repeat, where ROWS < kPer)
@@ -459,9 +457,13 @@ struct Split {
     int kvh, row_tile;
     int lim_ctx[NB], lim_new[NB];  // this lane's rows see cached keys below lim_ctx and fresh rows below lim_new
     uint64_t lane_off;             // of the KV head and of this lane's chunk, in a cache row
+    uint32_t my_offset;            // stage_offset()
+    const int32_t* table;          // the item's block-table row
 
     DFX_D Split(const SplitArgs& args, uint8_t* smem, float* ml_, int tid_)
-        : a(args), lds(smem), ml(ml_), tid(tid_), wave(uniform(tid_ >> 6)), lane(tid_ & 63), w(tid_ & 63) {}
+        : a(args), lds(smem), ml(ml_), tid(tid_), wave(uniform(tid_ >> 6)), lane(tid_ & 63), w(tid_ & 63) {
+        my_offset = stage_offset(lane, WIDE ? wave * ROWS : 0);
+    }
 
     // Key `lane` of tile t: look_up() loads its page's table entry, row_of() -- a tile later, so that nothing waits for the load --
     // makes it the byte offset of the key's cache row (token) and tells which keys have none: fresh tiles, keys behind the last,
@@ -476,7 +478,7 @@ struct Split {
         Key k;
         k.ok = t < sq.ctx_tiles && lane < KT && pos < sq.key1 && p < a.max_pages;
         k.off = pos - p * a.page_size;
-        k.page = a.block_tables[sq.table * a.bt_stride + min(p, a.max_pages - 1)];
+        k.page = table[static_cast<uint32_t>(min(p, a.max_pages - 1))];
         return k;
     }
     DFX_D int64_t row_of(const Key& k, uint64_t& valid) const {
@@ -491,6 +493,7 @@ struct Split {
         u32x4 w[kLoads];
         uint8_t s[kLoads];
     };
+    static DFX_D uint32_t address(const uint8_t* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); }
     // Which of a load's rows a lane takes.  A chunk of codes becomes 2 or 4 chunks in LDS, which leave one per lane at a time: 16 lanes
     // should then write all 16 chunk positions of a 256-byte LDS line, i.e. lie on rows whose swizzles (TileLayout) differ where their
     // chunk indices agree, in the lowest bits -- that is row bits 2 and 3.
@@ -517,9 +520,16 @@ struct Split {
             if constexpr (KV != kBf16) st.s[i] = scales[off >> (KV == kMx8 ? 5 : 4)];
         }
     }
+    // Byte offset in a tile in LDS of the first chunk that this lane writes of its load 0.  The chunks of a row and the rows of the other loads
+    // differ from it in bits that no carry reaches, so that the swizzle's XOR can be applied to the finished address (TileMath).
+    static constexpr int kWiden = KV == kBf16 ? 1 : KV == kMx8 ? 2 : 4;  // chunks in LDS per chunk of codes
+    static DFX_D uint32_t stage_offset(int lane, int r0) {
+        return L::chunk_offset(r0 + lane_row(lane / kChunks), lane % kChunks * kWiden);
+    }
     // Registers -> LDS, widened.  valid: which keys of the tile have a cache row.
     DFX_D void commit(Stage& st, uint8_t* to, int r0, uint64_t valid) const {
-        if (valid != kAll) {  // (a wave-uniform branch)
+        if (valid != kAll) {
+            asm volatile("");  // (a branch of the wave: as selects the zeroing would cost every tile)
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
                 if (!((valid >> ((r0 + stage_row(i)) & 63)) & 1)) {
@@ -527,24 +537,19 @@ struct Split {
                     st.s[i] = 0;
                 }
         }
-        int j = lane;
-        asm volatile("" : "+v"(j));  // (addresses worked out here: as invariants of the tile loop they take the registers of its tiles)
+        if (ROWS < kPer && stage_row(0) >= ROWS) return;
+        typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+        const uint32_t at = address(to) + my_offset;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int r = i * kPer + lane_row(j / kChunks), ch = j % kChunks;
-            if (ROWS < kPer && r >= ROWS) continue;
-            if constexpr (KV == kBf16) {
-                *reinterpret_cast<u32x4*>(to + L::chunk_offset(r0 + r, ch)) = st.w[i];
-            } else {
-                const float s = mx_scale_operand(st.s[i]);
-                constexpr int N = KV == kMx8 ? 2 : 4;
+            const float s = mx_scale_operand(st.s[i]);
 #pragma unroll
-                for (int x = 0; x < N; ++x) {
-                    u32x4 y;
-                    if constexpr (KV == kMx8) y = mx_widen8_e4m3(u32x2{st.w[i][2 * x], st.w[i][2 * x + 1]}, s);
-                    else y = mx_widen8_e2m1(st.w[i][x], s);
-                    *reinterpret_cast<u32x4*>(to + L::chunk_offset(r0 + r, ch * N + x)) = y;
-                }
+            for (int x = 0; x < kWiden; ++x) {
+                u32x4 y;
+                if constexpr (KV == kBf16) y = st.w[i];
+                else if constexpr (KV == kMx8) y = mx_widen8_e4m3(u32x2{st.w[i][2 * x], st.w[i][2 * x + 1]}, s);
+                else y = mx_widen8_e2m1(st.w[i][x], s);
+                *(lds_u32x4*)static_cast<uintptr_t>((at ^ ((x ^ L::swizzle(i * kPer)) * 16)) + i * kPer * L::ROWB) = y;
             }
         }
     }
@@ -560,7 +565,6 @@ struct Split {
         }
     }
     static DFX_D uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
-    static DFX_D uint32_t address(const uint8_t* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); }
 
     // Scores of the keys that a row does not see: of context tile t, of fresh tile t (counted from the first fresh one).
     template <int NT>
@@ -611,6 +615,7 @@ struct Split {
     }
     DFX_D void start_item(int rows_from, bool is_group) {
         lane_off = kvh * static_cast<uint64_t>(a.c_sh) + lane % kChunks * 16;
+        table = a.block_tables + sq.table * a.bt_stride;
         const bool uneven = uneven_group(is_group);
         w.reset();
         start_rows(0, rows_from, uneven);
@@ -649,8 +654,13 @@ struct Split {
     }
 
     // ---- wide ----------------------------------------------------------------------------------
-    // Context tiles: K runs a tile ahead of V; while the weights of tile u are made, the matrix pipeline makes the scores of
-    // u + 1.  Registers hold K of u + 2 and V of u + 1 on their way to LDS, the cache rows of u + 2 are known, those of u + 3 looked up.
+    // Context tiles, in two half steps each: (1) the weights of tile u from its scores, and beside them the scores of tile u + 1;
+    // (2) the outputs of tile u, and the wave's share of K of u + 3 and V of u + 2 from registers to LDS and of the tiles behind
+    // them from memory to registers.  The first is bound by the exponentials, the second by the matrix pipeline and by moving data:
+    // waves 4 to 7, which share their SIMDs with waves 0 to 3, run half a step behind, so that each SIMD has one wave in either.  (In step,
+    // the first half took 2100 cycles of a tile's 5100 and the wait at the barrier 1100.)
+    // What a half step reads was written two barriers before, and what it overwrites was read two barriers before, by the waves of
+    // either half: three buffers of K (scores of u + 1, u + 2, the one being written) and three of V.
     // No branch on the tile's kind in the loop and every wait for a step's loads before the next are issued: where a wait can be reached
     // with other loads in flight, the compiler waits for all of them.
     DFX_D void wide(int u0, int u1, bool is_group, int64_t slot, bool direct) {
@@ -658,66 +668,81 @@ struct Split {
         start_item(rows_from, is_group);
         const bool busy = rows_from < sq.rows;
         const int r0 = wave * ROWS;
-        auto k_buf = [&](int u) { return lds + ((u - u0) & 1) * kMat; };
-        auto v_buf = [&](int u) { return lds + (2 + ((u - u0) & 1)) * kMat; };
         const int c1 = min(u1, sq.ctx_tiles);
         if (u0 < c1) {
             Stage sk, sv;
             f32x16 s[2][NB];
             float top[NB];
-            int64_t row2;                     // cache rows of tile u + 2
-            Key key3;                         // keys of tile u + 3
-            uint64_t valid0, valid1, valid2;  // keys with a cache row of tiles u, u + 1, u + 2
+            int64_t row3;                             // cache rows of tile u + 3
+            Key key4;                                 // keys of tile u + 4
+            uint64_t valid0, valid1, valid2, valid3;  // keys with a cache row of tiles u, u + 1, ...
+            uint8_t *ka = lds, *kb = lds + kMat, *kc = lds + 2 * kMat;                  // K of u + 3 (and u), u + 1, u + 2
+            uint8_t *va = lds + 3 * kMat, *vb = lds + 4 * kMat, *vc = lds + 5 * kMat;  // V of u, u + 1, u + 2
             {
-                const Key key0 = look_up(u0), key1 = look_up(u0 + 1), key2 = look_up(u0 + 2);
-                key3 = look_up(u0 + 3);
-                const int64_t row0 = row_of(key0, valid0), row1 = row_of(key1, valid1);
-                row2 = row_of(key2, valid2);
+                const Key key0 = look_up(u0), key1 = look_up(u0 + 1), key2 = look_up(u0 + 2), key3 = look_up(u0 + 3);
+                key4 = look_up(u0 + 4);
+                const int64_t row0 = row_of(key0, valid0), row1 = row_of(key1, valid1), row2 = row_of(key2, valid2);
+                row3 = row_of(key3, valid3);
+                Stage k1, k2, v1;
                 issue(sk, a.k_cache, a.k_scales, row0, r0);
+                issue(k1, a.k_cache, a.k_scales, row1, r0);
                 issue(sv, a.v_cache, a.v_scales, row0, r0);
-                commit(sk, k_buf(u0), r0, valid0);
-                issue(sk, a.k_cache, a.k_scales, row1, r0);
-                commit(sv, v_buf(u0), r0, valid0);
-                issue(sv, a.v_cache, a.v_scales, row1, r0);
+                issue(k2, a.k_cache, a.k_scales, row2, r0);
+                issue(v1, a.v_cache, a.v_scales, row1, r0);
+                commit(sk, ka, r0, valid0);
+                commit(k1, kb, r0, valid1);
+                commit(sv, va, r0, valid0);
+                commit(k2, kc, r0, valid2);
+                commit(v1, vb, r0, valid1);
+                issue(sv, a.v_cache, a.v_scales, row2, r0);
+                issue(sk, a.k_cache, a.k_scales, row3, r0);
             }
             lds_barrier();
             if (busy) {
-                w.scores(address(k_buf(u0)), s);
+                w.scores(address(ka), s);
                 mask_context(s, u0, valid0);
                 top[0] = W::half_max(w.top_of(s, 0)) * a.c;
             }
-            commit(sk, k_buf(u0 + 1), r0, valid1);
-            issue(sk, a.k_cache, a.k_scales, row2, r0);
             lds_barrier();
+            const bool behind = wave >= kWgWaves / 2;
+            if (behind) lds_barrier();
             for (int u = u0; u + 1 < c1; ++u) {
-                const Key key4 = look_up(u + 4);
+                bf16x8 p[NB][2][2];
+                f32x16 next[2][NB];
+                const Key key5 = look_up(u + 5);
                 if (busy) {
-                    bf16x8 p[NB][2][2];
-                    f32x16 next[2][NB];
                     w.raise(0, top[0]);
-                    bf16x8 v[W::kAheadV + 1];
-                    w.weights_and_scores(s, a.c, p, address(k_buf(u + 1)), next, address(v_buf(u)), v);
+                    w.weights_and_scores(s, a.c, p, address(kb), next);
                     mask_context(next, u + 1, valid1);
-                    w.accumulate_and_top(address(v_buf(u)), p, next, top, v);
+                }
+                lds_barrier();
+                if (busy) {
+                    w.accumulate_and_top(address(va), p, next, top);
                     top[0] = W::half_max(top[0]) * a.c;
                     s[0][0] = next[0][0];
                     s[1][0] = next[1][0];
                 }
-                commit(sv, v_buf(u + 1), r0, valid1);
-                commit(sk, k_buf(u), r0, valid2);  // (of tile u + 2; behind the last, zeros that nobody reads)
-                issue(sv, a.v_cache, a.v_scales, row2, r0);
+                commit(sv, vc, r0, valid2);  // (of tiles u + 2 and u + 3; behind the last, zeros that nobody reads)
+                commit(sk, ka, r0, valid3);
+                issue(sv, a.v_cache, a.v_scales, row3, r0);
                 valid1 = valid2;
-                row2 = row_of(key3, valid2);
-                issue(sk, a.k_cache, a.k_scales, row2, r0);
-                key3 = key4;
+                valid2 = valid3;
+                row3 = row_of(key4, valid3);
+                issue(sk, a.k_cache, a.k_scales, row3, r0);
+                key4 = key5;
+                uint8_t* const k_old = ka;
+                uint8_t* const v_old = va;
+                ka = kb, kb = kc, kc = k_old;
+                va = vb, vb = vc, vc = v_old;
                 lds_barrier();
             }
             if (busy) {
                 bf16x8 p[NB][2][2];
                 w.raise(0, top[0]);
                 w.weights(s, a.c, p);
-                w.accumulate(address(v_buf(c1 - 1)), p);
+                w.accumulate(address(va), p);
             }
+            if (!behind) lds_barrier();
         }
         for (int u = max(u0, sq.ctx_tiles); u < u1; ++u) {
             const int t = u - sq.ctx_tiles;
