@@ -356,7 +356,7 @@ struct Wave {
     // the LDS operands requested some instructions ahead: an operand takes longer to arrive than a matrix instruction to run.
     // The scheduling barriers keep the source's order: left to itself the compiler puts the matrix instructions in a row (a wave waits at
     // the second until the first is through the pipeline), or all loads first, which does not fit the registers.
-    static constexpr int kAheadK = 2;  // slabs
+    static constexpr int kAheadK = 1;  // slabs
     static constexpr int kAheadV = 3;  // 16 keys x 32 elements each
     //   weights of s, scores of the next tile
     DFX_D void weights_and_scores(const f32x16 (&s)[2][NB], float c, bf16x8 (&p)[NB][2][2], uint32_t kt, f32x16 (&next)[2][NB]) {
@@ -512,12 +512,20 @@ struct Split {
     }
     // Issues the loads; `row` is row_of() the tile's keys.  No branch on the rows -- keys without a cache row load the cache's first
     // row and are zeroed in commit() -- so that the compiler can count the loads in flight.
-    DFX_D void issue(Stage& st, const uint8_t* codes, const uint8_t* scales, int64_t row, int r0) const {
+    struct Place {
+        uint64_t off[kLoads];
+    };
+    DFX_D Place place_of(int64_t row, int r0) const {
+        Place p;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) p.off[i] = static_cast<uint64_t>(shuffle64(row, r0 + min(stage_row(i), ROWS - 1))) + lane_off;
+        return p;
+    }
+    DFX_D void issue(Stage& st, const uint8_t* codes, const uint8_t* scales, const Place& p) const {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint64_t off = static_cast<uint64_t>(shuffle64(row, r0 + min(stage_row(i), ROWS - 1))) + lane_off;
-            st.w[i] = *reinterpret_cast<const u32x4*>(codes + off);
-            if constexpr (KV != kBf16) st.s[i] = scales[off >> (KV == kMx8 ? 5 : 4)];
+            st.w[i] = *reinterpret_cast<const u32x4*>(codes + p.off[i]);
+            if constexpr (KV != kBf16) st.s[i] = scales[p.off[i] >> (KV == kMx8 ? 5 : 4)];
         }
     }
     // Byte offset in a tile in LDS of the first chunk that this lane writes of its load 0.  The chunks of a row and the rows of the other loads
@@ -673,7 +681,7 @@ struct Split {
             Stage sk, sv;
             f32x16 s[2][NB];
             float top[NB];
-            int64_t row3;                             // cache rows of tile u + 3
+            Place at3;                                // of tile u + 3
             Key key4;                                 // keys of tile u + 4
             uint64_t valid0, valid1, valid2, valid3;  // keys with a cache row of tiles u, u + 1, ...
             uint8_t *ka = lds, *kb = lds + kMat, *kc = lds + 2 * kMat;                  // K of u + 3 (and u), u + 1, u + 2
@@ -681,21 +689,22 @@ struct Split {
             {
                 const Key key0 = look_up(u0), key1 = look_up(u0 + 1), key2 = look_up(u0 + 2), key3 = look_up(u0 + 3);
                 key4 = look_up(u0 + 4);
-                const int64_t row0 = row_of(key0, valid0), row1 = row_of(key1, valid1), row2 = row_of(key2, valid2);
-                row3 = row_of(key3, valid3);
+                const Place at0 = place_of(row_of(key0, valid0), r0), at1 = place_of(row_of(key1, valid1), r0);
+                const Place at2 = place_of(row_of(key2, valid2), r0);
+                at3 = place_of(row_of(key3, valid3), r0);
                 Stage k1, k2, v1;
-                issue(sk, a.k_cache, a.k_scales, row0, r0);
-                issue(k1, a.k_cache, a.k_scales, row1, r0);
-                issue(sv, a.v_cache, a.v_scales, row0, r0);
-                issue(k2, a.k_cache, a.k_scales, row2, r0);
-                issue(v1, a.v_cache, a.v_scales, row1, r0);
+                issue(sk, a.k_cache, a.k_scales, at0);
+                issue(k1, a.k_cache, a.k_scales, at1);
+                issue(sv, a.v_cache, a.v_scales, at0);
+                issue(k2, a.k_cache, a.k_scales, at2);
+                issue(v1, a.v_cache, a.v_scales, at1);
                 commit(sk, ka, r0, valid0);
                 commit(k1, kb, r0, valid1);
                 commit(sv, va, r0, valid0);
                 commit(k2, kc, r0, valid2);
                 commit(v1, vb, r0, valid1);
-                issue(sv, a.v_cache, a.v_scales, row2, r0);
-                issue(sk, a.k_cache, a.k_scales, row3, r0);
+                issue(sv, a.v_cache, a.v_scales, at2);
+                issue(sk, a.k_cache, a.k_scales, at3);
             }
             lds_barrier();
             if (busy) {
@@ -722,13 +731,16 @@ struct Split {
                     s[0][0] = next[0][0];
                     s[1][0] = next[1][0];
                 }
+                uint64_t valid4;
+                const Place at4 = place_of(row_of(key4, valid4), r0);
                 commit(sv, vc, r0, valid2);  // (of tiles u + 2 and u + 3; behind the last, zeros that nobody reads)
                 commit(sk, ka, r0, valid3);
-                issue(sv, a.v_cache, a.v_scales, row3, r0);
+                issue(sv, a.v_cache, a.v_scales, at3);
+                at3 = at4;
+                issue(sk, a.k_cache, a.k_scales, at3);
                 valid1 = valid2;
                 valid2 = valid3;
-                row3 = row_of(key4, valid3);
-                issue(sk, a.k_cache, a.k_scales, row3, r0);
+                valid3 = valid4;
                 key4 = key5;
                 uint8_t* const k_old = ka;
                 uint8_t* const v_old = va;
@@ -784,19 +796,19 @@ struct Split {
             for (int i = 0; i < kDepth; ++i) keys[i] = look_up(u + i * side);
 #pragma unroll
             for (int i = 0; i < kDepth; ++i) {
-                const int64_t row = row_of(keys[i], valid[i]);
+                const Place at = place_of(row_of(keys[i], valid[i]), 0);
                 keys[i] = look_up(u + (kDepth + i) * side);
-                issue(sk[i], a.k_cache, a.k_scales, row, 0);
-                issue(sv[i], a.v_cache, a.v_scales, row, 0);
+                issue(sk[i], a.k_cache, a.k_scales, at);
+                issue(sv[i], a.v_cache, a.v_scales, at);
             }
             auto step = [&](Stage& k, Stage& v, uint64_t& v_of, Key& key) {
                 commit(k, kt, 0, v_of);
                 commit(v, vt, 0, v_of);
                 const uint64_t here = v_of;
-                const int64_t row = row_of(key, v_of);
+                const Place at = place_of(row_of(key, v_of), 0);
                 key = look_up(u + 2 * kDepth * side);
-                issue(k, a.k_cache, a.k_scales, row, 0);
-                issue(v, a.v_cache, a.v_scales, row, 0);
+                issue(k, a.k_cache, a.k_scales, at);
+                issue(v, a.v_cache, a.v_scales, at);
                 asm volatile("" ::: "memory");  // (the tile is the wave's own: LDS keeps the wave's order)
                 whole_tile(kt, vt, [&](auto& s) { mask_context(s, u, here); });
                 asm volatile("" ::: "memory");
