@@ -34,7 +34,9 @@ constexpr int kNarrowMost = 96;  // rows of a virtual sequence up to which its i
 // Beside its units (cost 1 each) an item costs its start and end: queries, first tiles, the merge of the waves, the rows written.
 // (Narrow: of the tiles that the waves of a head take side by side; a unit is one such tile.)
 constexpr int kNarrowTail = 2, kWideTail = 3;
-constexpr int kNarrowLeast = 2, kWideLeast = 2;  // least cost per workgroup
+// Least cost per workgroup.  Shorter pieces take the merge longer than they save: 64 single tokens with a prefix of 4096 take 70, 66, 68 us with 2, 4, 6 for
+// the wide, 8 tokens over 100 to 1000 keys 24.5, 25.7, 27.1 us with 2, 3, 4 for the narrow ones.
+constexpr int kNarrowLeast = 2, kWideLeast = 4;
 
 enum { kBf16 = 0, kMx8 = 1, kMx4 = 2 };
 
@@ -909,6 +911,15 @@ DFX_D Seq uniform_seq(const Seq& s) {  // (what LDS returns is a vector register
                uniform(s.narrow) != 0, uniform(s.group)};
 }
 
+// Number of the i-th of `launched` workgroups among the `n_wg` that work (n_wg or more: none).  Workgroups go to the eight XCDs in turn: neighbouring
+// ranges (the row tiles that read the same keys) are to be on one of them.
+DFX_D int numbered(int i, int launched, int n_wg) {
+    const int xcd = i % 8, slot = i / 8, each = launched / 8;
+    if (n_wg > each * 8) return xcd * each + min(xcd, launched % 8) + slot;  // (all of them, the last round of the XCDs is not full)
+    const int used = (n_wg + 7) / 8;
+    return slot < used ? xcd * used + slot : n_wg;
+}
+
 template <int HD, int KV, bool WIDE>
 __global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(const SplitArgs a) {
     using T = Split<HD, KV, WIDE>;
@@ -963,9 +974,7 @@ __global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(con
         if (!WIDE && tid == 0) comb[a.n_seqs] = total.comb;
         return;
     }
-    // neighbouring ranges (the row tiles that read the same keys) on one XCD: workgroups go to the eight in turn
-    const int slot_in = static_cast<int>(blockIdx.x - 1) / 8, per_xcd = (n_wg + 7) / 8;
-    const int wg = slot_in < per_xcd ? static_cast<int>(blockIdx.x - 1) % 8 * per_xcd + slot_in : n_wg;
+    const int wg = numbered(static_cast<int>(blockIdx.x - 1), a.n_wg[WIDE], n_wg);
     if (wg >= n_wg || total.cost == 0) return;
     const int64_t c0 = range_start(wg, total.cost, n_wg), c1 = range_start(wg + 1, total.cost, n_wg);
     if (c0 >= c1) return;

@@ -446,3 +446,50 @@ def test_nothing_to_do(dev):
                         prefix_cu_seqs=torch.zeros(1, dtype=torch.int32, device=dev), prefix_lens=torch.zeros(0, dtype=torch.int32, device=dev))
     torch.cuda.synchronize()
     no_cache.check(out.cpu())
+
+
+@pytest.mark.parametrize("n_wg", [7, 9, 10, 13, 15, 37, 100])
+def test_numbers_of_workgroups_that_the_dies_do_not_share_evenly(dev, n_wg):
+    """No range of the work may be left without a workgroup."""
+    p = Problem("e2m1", [900, 650, 40, 1200], [1, 20, 3, 1], 28, 4, 128, 32, seed=6, groups=[(0, 2, 600)])
+    p.check(p.run(dev, max_workgroups=n_wg))
+
+
+@pytest.mark.parametrize("batch,groups", [(300, 0), (700, 0), (640, 600), (1100, 3)])
+def test_more_virtual_sequences_than_threads(dev, batch, groups):
+    """A thread then lists several of them, and the merge looks a row block's up among several per thread (from 1025 blocks on with four waves)."""
+    ctx = [(s * 37) % 61 + (8 if groups else 0) for s in range(batch)]
+    new = [(s * 7) % 4 for s in range(batch)]
+    each = max(batch // groups, 1) if groups else 0
+    p = Problem("e4m3", ctx, new, 4, 2, 64, 8, seed=7, groups=[(g * each, (g + 1) * each, 8) for g in range(groups)])
+    p.check(p.run(dev))
+
+
+def test_narrow_and_wide_items_side_by_side(dev):
+    p = Problem("bf16", [50, 10, 900] * 20, [1, 3, 20] * 20, 28, 4, 128, 32, seed=8, groups=[(0, 20, 7)])
+    want = p.want()
+    for n_wg in (0, 2, 12):
+        p.check(p.run(dev, max_workgroups=n_wg), want)
+
+
+def test_two_calls_at_once_on_two_streams(dev):
+    """Each call has a workspace of its own."""
+    a = Problem("e4m3", [400, 900, 33], [5, 1, 2], 28, 4, 128, 32, seed=9)
+    b = Problem("e2m1", [1300, 64], [40, 7], 8, 2, 64, 16, seed=10)
+    wa, wb = a.want(), b.want()
+    ma, mb = a.metadata(dev), b.metadata(dev)
+    on = lambda p: [x.to(dev) for x in (p.q, p.k, p.v, p.kc, p.vc)]  # noqa: E731
+    ta, tb, sa, sb = on(a), on(b), a.scales(dev), b.scales(dev)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(one):
+            ga = dfx.dllm_flash_attn_decode(*ta, a.scale, ma, **sa)
+        with torch.cuda.stream(two):
+            gb = dfx.dllm_flash_attn_decode(*tb, b.scale, mb, **sb)
+        got.append((ga, gb))
+    torch.cuda.synchronize()
+    for ga, gb in got:
+        a.check(ga.cpu(), wa)
+        b.check(gb.cpu(), wb)
