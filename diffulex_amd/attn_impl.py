@@ -38,6 +38,7 @@ class Attention(nn.Module):
         where a store is due."""
         stored = False
         mx = _is_block_scale(self.k_scale)
+        assert not mx or self.fetch_attn_metadata().kv_cache_layout == "unified", "microscaled caches have the unified layout"
         if rope is not None:
             rotary, positions = rope
             md = self.fetch_attn_metadata()

@@ -130,7 +130,8 @@ DFX_D int group_of(const SplitArgs& a, int s) {
 DFX_D Seq seq_of(const SplitArgs& a, int v) {
     Seq q;
     const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size;
-    const int cap = static_cast<int>(capacity > INT32_MAX - 64 ? INT32_MAX - 64 : capacity);
+    // (keys are numbered in 32 bits, those of the tiles looked up ahead, up to 832 behind the last key, included)
+    const int cap = static_cast<int>(capacity > INT32_MAX - 1024 ? INT32_MAX - 1024 : capacity);
     q.new0 = q.n_new = 0;
     q.group = -1;
     if (v < a.n_groups) {

@@ -93,6 +93,8 @@ def paged_attention(q, k, v, k_cache, v_cache, scale, *, block_tables, context_l
     contexts; they are read once for all of them, through the first one's block-table row (bf16 or microscaled caches in
     the unified layout).  The fused forms -- ``rope``, ``static_scratch`` -- are not offered there; ``store_slot_mapping`` is,
     as a launch of its own behind the attention."""
+    if (prefix_lens is None) != (prefix_cu_seqs is None):
+        raise _lib.DfxError("dfx_split_attn: prefix_cu_seqs and prefix_lens go together (invalid argument)")
     if prefix_lens is not None or _is_block_scale(k_scale):
         if rope is not None or static_scratch or cache_layout != "unified":
             raise _lib.DfxError("dfx_split_attn: microscaled caches and shared prefixes take the unified layout, without rope and "
@@ -184,6 +186,8 @@ def _split_attention(q, k, v, k_cache, v_cache, scale, block_tables, context_len
     key = (q.device.index, q.shape, k.shape[1], num_seqs, groups, max_workgroups, max_seqlen_q)
     need = _split_need.get(key)
     if need is None:
+        if len(_split_need) >= 4096:
+            _split_need.clear()
         need = _split_need[key] = int(_call(ops.split_attention_workspace_bytes, q, k.shape[1], num_seqs, groups, int(max_workgroups),
                                                 int(max_seqlen_q)))
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -53,6 +53,10 @@ def _scaled_frequencies(dim: int, max_position: int, base: float, scaling: Optio
     kind = scaling.get("rope_type", scaling.get("type"))
     if kind not in ("linear", "dynamic", "yarn"):
         raise ValueError(f"unknown rope_scaling {scaling!r}")
+    known = {"rope_type", "type", "factor", "original_max_position_embeddings"}
+    unknown = sorted(set(scaling) - known - ({"beta_fast", "beta_slow", "attention_factor"} if kind == "yarn" else set()))
+    if unknown:  # (a setting left out would give other angles than the model was trained with)
+        raise ValueError(f"rope_scaling {kind!r} has no {', '.join(unknown)}")
     factor = float(scaling["factor"])
     if not (factor >= 1.0 and math.isfinite(factor)):
         raise ValueError(f"rope_scaling factor {factor} is not a finite number >= 1")

@@ -136,7 +136,8 @@ int dfx_kv_load(const void* k_cache, const void* v_cache, const void* k_new, con
  * of 32 elements x of a key or value head row with largest magnitude A, the store writes the scale byte b = 127 + e, e
  * the smallest integer >= -127 with A <= M * 2^e (M = 448 for E4M3, 6 for E2M1), and for each element the code nearest to
  * x * 2^-e (ties to even).  A block with an infinity or NaN gets b = 255 (it reads back as NaN) and codes 0.
- * Slots as in dfx_kv_store_unified (slots < 0 or >= n_slots are skipped).
+ * Slots as in dfx_kv_store_unified (slots < 0 or >= n_slots are skipped; a slot is given at most once: of two rows for one
+ * slot the codes may be one's and the scales the other's).
  *
  * dfx_kv_load_mx gathers like dfx_kv_load but widens to bf16 (exactly: a code has at most 4 significant bits): rows
  * [cu_seqlens_k[s], + context_lens[s]) of k_out / v_out ([n_out, n_kv_heads, head_dim] bf16, dense) from the cache, then
@@ -522,13 +523,14 @@ int dfx_rope_kv_store(const dfx_rope_params* params, dfx_stream_t stream);
  *
  * Groups (num_groups > 0): sequences prefix_cu_seqs[g] .. prefix_cu_seqs[g + 1) -- neighbours in the batch; sequences before the
  * first or behind the last group have no shared prefix -- hold the same keys at positions [0, prefix_lens[g]) of
- * their contexts, which are read ONCE for all of them, through the block table of the group's first sequence; every
+ * their contexts, which are read ONCE for all of them, through the block table of the group's first sequence (whose row
+ * holds the pages of all prefix_lens[g] positions, also where its own context is shorter); every
  * sequence's keys from prefix_lens[g] on come through its own table row.  The other sequences' table entries below
  * prefix_lens[g] / page_size are not read.  A sequence whose context is shorter than its group's prefix sees its context_lens keys
  * of it.
  *
- * Two or three launches (pieces, merge), planned on the device from the lengths: nothing is read back, both may be recorded into a
- * graph whose replays find other lengths, and the results do not depend on timing (pieces are merged in order).  The workspace
+ * Two or three launches (pieces of many rows, pieces of few, merge), planned on the device from the lengths: nothing is read back, they
+ * may be recorded into a graph whose replays find other lengths, and the results do not depend on timing (pieces are merged in order).  The workspace
  * (dfx_split_attn_workspace_bytes(), 256-byte aligned, any contents) must not be shared by calls that overlap in time.
  *
  * Supported: head_dim 64 or 128; num_q_heads a multiple of num_kv_heads; any page_size >= 1; num_seqs <= 65535; strides in

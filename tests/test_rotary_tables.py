@@ -107,3 +107,13 @@ def test_mx_entry_points_refuse_without_launching():
     for bad, status in ((dict(fmt=1), -1), (dict(hd=48), -2), (dict(ks=120), -1), (dict(ks=132), -1), (dict(key=4098), -1), (dict(type=2), -1),
                         (dict(vsc=None), -1), (dict(n=-1), -1), (dict(heads=0), -1), (dict(n=1 << 40), -2)):
         assert store(**bad) == status, bad
+
+
+@pytest.mark.parametrize("extra", [dict(mscale=0.7), dict(truncate=False), dict(low_freq_factor=1.0)])
+@pytest.mark.parametrize("kind", ["linear", "dynamic", "yarn"])
+def test_settings_that_are_not_understood_are_refused(kind, extra):
+    with pytest.raises(ValueError, match=next(iter(extra))):
+        RotaryEmbedding(64, 64, 32, 1e4, rope_scaling=dict(rope_type=kind, factor=2.0, **extra))
+    if kind != "yarn":
+        with pytest.raises(ValueError, match="beta_fast"):
+            RotaryEmbedding(64, 64, 32, 1e4, rope_scaling=dict(rope_type=kind, factor=2.0, beta_fast=16))

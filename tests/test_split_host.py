@@ -2,10 +2,12 @@
 import ctypes as C
 import os
 import subprocess
+import types
 
 import pytest
 import torch
 
+import diffulex_amd as dfx
 from diffulex_amd import _lib
 from oracle import attention as oat
 from oracle import split
@@ -74,3 +76,21 @@ def test_oracle_agrees_with_the_fp32_oracle(block_causal):
                                     mask_mode=int(block_causal), dbs=4)
     # fp32 sums of 64 products and of at most 42 weights: a few thousand steps of 2^-24 at most
     assert (got - want.double()).abs().max() < 1e-4 and written.all() and (spread >= got.abs() - 1e-12).all()
+
+
+def test_half_a_pair_of_prefix_tensors_is_refused():
+    x, one = torch.zeros(1, 1, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    for kw in (dict(prefix_cu_seqs=one), dict(prefix_lens=one[:1])):
+        with pytest.raises(_lib.DfxError, match="go together"):
+            dfx.paged_attention(x, x, x, None, None, 1.0, block_tables=None, context_lens=None, cu_seqlens_q=one, cu_seqlens_new=one,
+                                max_seqlen_q=1, **kw)
+
+
+def test_microscaled_caches_in_the_distinct_layout_are_refused():
+    md = types.SimpleNamespace(is_prefill=False, kv_cache_layout="distinct")
+    layer = dfx.Attention(1, 64, 1.0, 1)
+    layer.k_scale = layer.v_scale = torch.zeros(2, 8, 1, 2, dtype=torch.uint8)
+    layer.fetch_attn_metadata = lambda: md
+    x = torch.zeros(1, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="unified"):
+        layer(x, x, x)
