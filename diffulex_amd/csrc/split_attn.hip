@@ -18,8 +18,13 @@
 //     four (a token's codes and scales of neighbouring heads lie in the same memory lines: the waves of a workgroup should want them
 //     at the same time), with every second or fourth tile of a head otherwise, whose softmax states are then merged in LDS.
 //     A wave moves its 32-key tiles into LDS of its own: no barrier in the loop, the next tiles' loads in flight over the arithmetic.
+//     5 single tokens of 32 / 32 heads over 20000 to 60000 E2M1 keys: 274 us, 3.0 TB/s (425 us with a workgroup's waves on four tiles of one
+//     head: a head's 4 scale bytes and 64 codes are a part of a memory line each).
 //   wide: bound by the matrix instructions and the exponentials.  256 rows, 32 for each of eight waves, over 64-key tiles shared by the
 //     waves; in each wave the products of one tile's scores run beside the exponentials of the tile before.
+//     128 sequences of 32 tokens, 28 / 4 heads, over 2048 to 8192 E4M3 keys: 420 to 455 us, 680 to 735 TFLOP/s of the rows' own products (224 of a tile's
+//     256 rows).  Two row blocks per wave (half the LDS reads) do not fit the registers; one launch for both kinds, sharing the workgroups out,
+//     gained 7 us where a prefix of 4096 serves 64 single tokens and lost 8 to 17 us elsewhere.
 // Microscaled codes are widened on the way from registers to LDS, once per tile, with their block's scale applied by the same
 // instruction: from there on the arithmetic is the bf16 cache's.
 #include "attn_tile.h"
@@ -30,7 +35,7 @@ namespace {
 
 constexpr int kNarrowRows = 32, kWideRows = 256;
 constexpr int kNarrowKeys = 32, kWideKeys = 64;
-constexpr int kNarrowMost = 96;  // rows of a virtual sequence up to which its items are narrow
+constexpr int kNarrowMost = 96;  // rows of a virtual sequence up to which its items are narrow: three tiles of 32, which read the keys three times
 // Beside its units (cost 1 each) an item costs its start and end: queries, first tiles, the merge of the waves, the rows written.
 // (Narrow: of the tiles that the waves of a head take side by side; a unit is one such tile.)
 constexpr int kNarrowTail = 2, kWideTail = 3;
