@@ -35,7 +35,10 @@ namespace {
 
 constexpr int kNarrowRows = 32, kWideRows = 256;
 constexpr int kNarrowKeys = 32, kWideKeys = 64;
-constexpr int kNarrowMost = 96;  // rows of a virtual sequence up to which its items are narrow: three tiles of 32, which read the keys three times
+// Rows of a virtual sequence up to which its items are narrow.  Each tile of 32 rows reads the keys again, a wide tile costs the same whatever its rows.
+// (Narrow against wide, E4M3, 4 KV heads, us: 32 rows over 4096 keys, 64 sequences: 110, 123; 64 rows: 143, 137; 96 rows: 219, 141, a bf16 cache 356,
+// 176; 96 rows, 4 sequences: 47, 38; 64 rows over 700 keys, 128 sequences: 79, 87; 84 rows over 16 to 700 keys beside 4 prefixes of 8192: 320, 337.)
+constexpr int kNarrowMost = 32;
 // Beside its units (cost 1 each) an item costs its start and end: queries, first tiles, the merge of the waves, the rows written.
 // (Narrow: of the tiles that the waves of a head take side by side; a unit is one such tile.)
 constexpr int kNarrowTail = 2, kWideTail = 3;
@@ -1041,8 +1044,9 @@ __global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(con
 // kAtOnce of them together.  Bound by latency: the list and the pieces lie in memory that another XCD wrote, so everything that may be
 // needed of the list is asked for at once.  (The order of the sums is the pieces', whoever finished first.)
 constexpr int kAtOnce = 4;
-// Few row blocks have many pieces each (the work is spread over all workgroups), many have few.
-constexpr int kMergeWavesFew = 16, kMergeWavesMany = 4, kFewBlocks = 1024;
+// Few row blocks have many pieces each (the work is spread over all workgroups), many have few.  (Whole calls with 4 and with 16 waves, us: 256 blocks 43,
+// 34; 800 blocks 56, 61; 2048 blocks 80, 102.)
+constexpr int kMergeWavesFew = 16, kMergeWavesMany = 4, kFewBlocks = 512;
 
 template <int HD, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64) split_merge_kernel(const SplitArgs a) {
