@@ -1234,7 +1234,6 @@ int lay_out(const dfx_split_attn_params* p, SplitArgs& a, int64_t& comb_blocks, 
     // (an item of R rows takes at most R / 32 + 1 slots if it is narrow, R / 32 + 8 if it is wide, which needs more than kNarrowMost rows)
     const int64_t copies = (p->num_groups > 0 ? 2 : 1) * rows32;
     const int64_t wide_vs = vs < copies * 32 / kNarrowMost ? vs : copies * 32 / kNarrowMost;
-    // (and chunks of at least a workgroup's share add at most an item per workgroup; a piece's slot is its workgroup's and its item's index)
     a.heads_shift = a.h_kv % 4 == 0 ? 2 : a.h_kv % 2 == 0 ? 1 : 0;
     // (a piece's slot is the sum of its workgroup's and its item's index)
     a.n_slots[0] = (static_cast<int64_t>(a.n_wg[0]) << a.heads_shift) + a.h_kv * (copies + vs);
