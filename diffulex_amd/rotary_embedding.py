@@ -169,6 +169,13 @@ class RotaryEmbedding(nn.Module):
         return q_out, k_out
 
 
+def _frozen(x):
+    """A dict, list or tuple as nested tuples that a cache can be keyed with."""
+    if isinstance(x, dict):
+        return tuple(sorted((k, _frozen(v)) for k, v in x.items()))
+    return tuple(_frozen(v) for v in x) if isinstance(x, (list, tuple)) else x
+
+
 @lru_cache(1)
 def _get_rope(head_size, rotary_dim, max_position, base, rope_scaling, is_neox_style):
     return RotaryEmbedding(head_size, rotary_dim, max_position, base, is_neox_style,
@@ -179,4 +186,8 @@ def get_rope(head_size: int, rotary_dim: int, max_position: int, base: float,
              rope_scaling: dict | None = None, is_neox_style: bool = True):
     """rotary_embedding.py:69-79 (one module, kept until other arguments are asked for)."""
     return _get_rope(head_size, rotary_dim, max_position, base,
-                     tuple(sorted(rope_scaling.items())) if rope_scaling is not None else None, bool(is_neox_style))
+                     _frozen(rope_scaling) if rope_scaling is not None else None, bool(is_neox_style))
+
+
+# what the cached function of the reference offers besides the call
+get_rope.cache_info, get_rope.cache_clear = _get_rope.cache_info, _get_rope.cache_clear

@@ -117,3 +117,17 @@ def test_settings_that_are_not_understood_are_refused(kind, extra):
     if kind != "yarn":
         with pytest.raises(ValueError, match="beta_fast"):
             RotaryEmbedding(64, 64, 32, 1e4, rope_scaling=dict(rope_type=kind, factor=2.0, beta_fast=16))
+
+
+def test_get_rope_is_still_a_cache():
+    a = get_rope(64, 64, 16, 1e4)
+    assert get_rope.cache_info().currsize == 1
+    get_rope.cache_clear()
+    assert get_rope.cache_info().currsize == 0 and get_rope(64, 64, 16, 1e4) is not a
+
+
+def test_settings_with_lists_reach_the_constructor():
+    with pytest.raises(ValueError, match="unknown rope_scaling"):
+        get_rope(64, 64, 16, 1e4, dict(rope_type="other", short_factor=[1.0, 2.0], nested=dict(a=[1])))
+    with pytest.raises(ValueError, match="short_factor"):
+        get_rope(64, 64, 16, 1e4, dict(rope_type="yarn", factor=2.0, short_factor=[1.0, 2.0]))
