@@ -3,13 +3,16 @@
 //   code value c, scale byte b:  element = c * 2^(b - 127)          (b == 255: the block is NaN)
 //   E4M3 codes (one byte, largest magnitude M = 448) or E2M1 codes (four bits, M = 6; element 2 i in the low half of byte i).
 //   Writing a block with largest magnitude A: b - 127 = the smallest e with A <= M 2^e (at least -127), codes = the multiples
-//   of the code's grid nearest to x 2^-e, ties to even.  A block that holds an infinity or NaN gets b = 255 and codes 0.
+//   of the code's grid nearest to x 2^-e, ties to even, among those whose element is below 2^128 (MxLast).  A block that holds
+//   an infinity or NaN gets b = 255 and codes 0.
 //
-// With a power of two as the scale, x 2^-e is exact in fp32 (the codes round once, from the exact quotient), and
-// code * scale, 4 or 2 significant bits, is exactly a bf16: widening loses nothing and the matrix instructions see what the
-// cache holds.  gfx950 converts two codes and applies the scale in one instruction (v_cvt_scalef32_pk_bf16_fp8 / _fp4), whose
-// scale operand is read as its exponent field: the byte shifted to bit 23 is the E8M0 scale for all 256 bytes (byte 0 is
-// 2^-127, byte 255 NaN) -- compared with 64-bit arithmetic for every byte and every code.
+// With a power of two as the scale, x 2^-e is exact in fp32 (the codes round once, from the exact quotient), and every
+// code * scale that a finite block is written with, 4 or 2 significant bits, is exactly a finite bf16 (a subnormal one too: x is a
+// multiple of 2^-133, and so is what it is rounded to): widening loses nothing and the matrix instructions see what the cache
+// holds.  Codes and scales from elsewhere may stand for elements that bf16 has not: those below its smallest subnormal are rounded,
+// those from 2^128 on are infinities.  gfx950 converts two codes and applies the scale in one instruction
+// (v_cvt_scalef32_pk_bf16_fp8 / _fp4), whose scale operand is read as its exponent field: the byte shifted to bit 23 is the
+// E8M0 scale for all 256 bytes (byte 0 is 2^-127, byte 255 NaN) -- compared with 64-bit arithmetic for every byte and every code.
 #pragma once
 
 #include "dfx_common.h"
@@ -51,9 +54,18 @@ DFX_D uint32_t max_quad(uint32_t v) {
     return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xf, 0xf, true)));  // lanes 2 3 0 1
 }
 
+// The scale byte of blocks whose largest magnitudes round up to a code that stands for 2^128 (255 to 256 with 2^120, 3.98 to 4 with 2^126),
+// and the last code whose element is a finite bf16.  (Blocks of smaller maxima have smaller bytes, and M 2^e below 2^128.)
+template <bool E2M1>
+struct MxLast {
+    static constexpr uint32_t kByte = E2M1 ? 253 : 247;
+    static constexpr float kCode = E2M1 ? 3.0f : 240.0f;
+};
+
 // 2^-e as a float for scale byte b (0 for the byte of a non-finite block: its codes are written as zeros).
 DFX_D float mx_inverse_scale(uint32_t b) { return b == 255u ? 0.0f : __builtin_bit_cast(float, (254u - b) << 23); }
 
+template <bool E2M1>
 DFX_D void mx_scaled8(u32x4 w, uint32_t scale_byte, float (&y)[8]) {
     const float s = mx_inverse_scale(scale_byte);
     const bool bad = scale_byte == 255u;
@@ -64,12 +76,16 @@ DFX_D void mx_scaled8(u32x4 w, uint32_t scale_byte, float (&y)[8]) {
         y[2 * i] = bad ? 0.0f : lo;  // (an infinity times 0 would be a NaN)
         y[2 * i + 1] = bad ? 0.0f : hi;
     }
+    if (scale_byte == MxLast<E2M1>::kByte) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(y[i], -MxLast<E2M1>::kCode, MxLast<E2M1>::kCode);
+    }
 }
 
 // 8 bf16 -> 8 E4M3 codes.  v_cvt_pk_fp8_f32 rounds to nearest even (compared with a library cast for all bf16 up to 448).
 DFX_D u32x2 mx_codes8_e4m3(u32x4 w, uint32_t scale_byte) {
     float y[8];
-    mx_scaled8(w, scale_byte, y);
+    mx_scaled8<false>(w, scale_byte, y);
     u32x2 r;
     int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     r.x = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], v, true));
@@ -81,7 +97,7 @@ DFX_D u32x2 mx_codes8_e4m3(u32x4 w, uint32_t scale_byte) {
 // 8 bf16 -> 8 E2M1 codes (a dword).
 DFX_D uint32_t mx_codes8_e2m1(u32x4 w, uint32_t scale_byte) {
     float y[8];
-    mx_scaled8(w, scale_byte, y);
+    mx_scaled8<true>(w, scale_byte, y);
     uint32_t r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[2], y[3], 1.0f, 1);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[4], y[5], 1.0f, 2);

@@ -135,11 +135,13 @@ int dfx_kv_load(const void* k_cache, const void* v_cache, const void* k_new, con
  * DFX_KV_MX_E2M1); k_scales / v_scales: [n_slots, n_kv_heads, head_dim / 32] E8M0 bytes, dense.  For each block
  * of 32 elements x of a key or value head row with largest magnitude A, the store writes the scale byte b = 127 + e, e
  * the smallest integer >= -127 with A <= M * 2^e (M = 448 for E4M3, 6 for E2M1), and for each element the code nearest to
- * x * 2^-e (ties to even).  A block with an infinity or NaN gets b = 255 (it reads back as NaN) and codes 0.
+ * x * 2^-e (ties to even; among the codes that stand for less than 2^128: what is finite stays finite).  A block with an infinity or
+ * NaN gets b = 255 (it reads back as NaN) and codes 0.
  * Slots as in dfx_kv_store_unified (slots < 0 or >= n_slots are skipped; a slot is given at most once: of two rows for one
  * slot the codes may be one's and the scales the other's).
  *
- * dfx_kv_load_mx gathers like dfx_kv_load but widens to bf16 (exactly: a code has at most 4 significant bits): rows
+ * dfx_kv_load_mx gathers like dfx_kv_load but widens to bf16 (exactly for whatever a store wrote: a code has at most 4 significant
+ * bits; other codes and scales may stand for less than bf16's smallest subnormal, and are rounded, or for 2^128 and more: infinities): rows
  * [cu_seqlens_k[s], + context_lens[s]) of k_out / v_out ([n_out, n_kv_heads, head_dim] bf16, dense) from the cache, then
  * seq_lens_new[s] rows of k_new / v_new ([n_new, ..] bf16) as they are.  Rows of skipped pages (table entry < 0 or
  * >= n_pages) and rows at or beyond n_out are not written; fresh rows at or beyond n_new are not read.

@@ -2,7 +2,8 @@
 
 A block is 32 consecutive elements of a head row.  Definition (include/diffulex_amd.h, ``dfx_kv_store_mx``): scale exponent
 e = the smallest integer >= -127 with A <= M 2^e for the block's largest magnitude A, codes nearest to x 2^-e with ties to
-the even code; element = code value * 2^e.  A block with an infinity or NaN has scale byte 255 and codes 0.  Pinned in
+the even code, among those whose magnitude times 2^e is below 2^128; element = code value * 2^e.  A block with an infinity or NaN
+has scale byte 255 and codes 0.  Pinned in
 tests/test_oracle_mx.py against library casts, a brute-force search over all code values and the grids written out.
 """
 from __future__ import annotations
@@ -55,6 +56,8 @@ def quantise(x: torch.Tensor, fmt: str):
     code = np.searchsorted(mid, a, side="left")      # number of midpoints below a: a tie stays at the lower code
     tie = (code < len(mid)) & (a == mid[np.minimum(code, len(mid) - 1)])
     code = np.where(tie & (code % 2 == 1), code + 1, code)
+    last = np.searchsorted(pos, np.where(s > 0, 2.0 ** 128 / np.where(s > 0, s, 1.0), np.inf), side="left") - 1  # the largest below 2^128 / s
+    code = np.minimum(code, last)
     code = np.where(np.signbit(y), code + half, code)
     code = np.where((b == 255)[..., None], 0, code)
     return torch.from_numpy(code.reshape(xd.shape).astype(np.uint8)), torch.from_numpy(b)

@@ -202,3 +202,52 @@ def test_store_recorded_into_a_graph_and_on_another_stream(dev):
         torch.cuda.synchronize()
         codes, b = mx.quantise(r.cpu(), "e4m3")
         assert torch.equal(kc.cpu().flatten(0, 1)[slots.cpu().long()], codes) and torch.equal(ks.cpu().flatten(0, 1)[slots.cpu().long()], b)
+
+
+def _load_all(kc, vc, ks, vs, dev):
+    """Every row of a cache, loaded as one context."""
+    m = _MD()
+    n = kc.shape[0] * kc.shape[1]
+    i32 = dict(dtype=torch.int32, device=dev)
+    m.block_tables, m.context_lens = torch.arange(kc.shape[0], **i32)[None], torch.tensor([n], **i32)
+    m.seq_lens_ts, m.seq_lens, m.max_seqlen_k = torch.zeros(1, **i32), None, n
+    m.cu_seqlens_q, m.cu_seqlens_k = torch.zeros(2, **i32), torch.tensor([0, n], **i32)
+    none = torch.empty(0, kc.shape[2], ks.shape[3] * 32, dtype=torch.bfloat16, device=dev)
+    out = dfx.load_kvcache(kc.to(dev), vc.to(dev), m, none, none, k_scale=ks.to(dev), v_scale=vs.to(dev))
+    torch.cuda.synchronize()
+    return tuple(x.cpu() for x in out)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_load_every_scale_and_code(dev, fmt):
+    """All 256 scale bytes with all codes: code * 2^(b - 127) rounded to bf16 (which it is already, but for products below bf16's smallest
+    subnormal), 2^128 and more an infinity."""
+    codes = 256 if fmt == "e4m3" else 16
+    rows = max(codes // 32, 1)
+    c = torch.arange(codes).repeat(32 // min(codes, 32)).view(rows, 32).to(torch.uint8).repeat(256, 1)
+    kc = mx.pack(c, fmt).reshape(-1, 8, 1, 32 if fmt == "e4m3" else 16)
+    ks = torch.arange(256, dtype=torch.uint8).repeat_interleave(rows).view(-1, 8, 1, 1)
+    want = mx.values(kc, ks, fmt).flatten(0, 1).to(torch.bfloat16)
+    for got in _load_all(kc, kc.clone(), ks, ks.clone(), dev):
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        ok = ~torch.isnan(want)
+        assert torch.equal(got.view(torch.int16)[ok], want.view(torch.int16)[ok])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_every_finite_bf16_stored_and_loaded_is_finite(dev, fmt):
+    """What a store writes is a bf16 for every finite row: the load widens it exactly.  Up to half a step of the code's grid from the row, or one step in
+    the last binade, where the nearest code would stand for 2^128."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    bits = bits[torch.isfinite(bits)]
+    n = bits.numel()                                       # 65280 = 4080 pages of 16
+    x = torch.zeros(n, 2, 32, dtype=torch.bfloat16)
+    x[:, 0, 3] = bits
+    x[:, 1, 11], x[:, 1, 30] = bits, 1.75
+    kc, vc, ks, vs = _empty(fmt, n // 16, 16, 2, 32, dev)
+    g = x.to(dev)
+    dfx.store_kvcache_unified_layout(g, -g, kc, vc, torch.arange(n, dtype=torch.int32, device=dev), None, k_scale=ks, v_scale=vs)
+    got, negated = _load_all(kc, vc, ks, vs, dev)
+    assert torch.isfinite(got).all() and torch.equal(negated.double(), -got.double())
+    codes, b = mx.quantise(x, fmt)
+    assert torch.equal(got.double(), mx.values(mx.pack(codes, fmt), b, fmt))

@@ -69,3 +69,19 @@ def test_non_finite_blocks_are_nan(fmt):
     assert (b == 255).tolist() == [[True, False, False], [False, True, False], [False, False, True]]
     v = mx.values(mx.pack(codes, fmt), b, fmt)
     assert torch.isnan(v[0, :32]).all() and (v[0, 32:] == 1).all() and torch.isnan(v[1, 32:64]).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_finite_rows_have_finite_bf16_values(fmt):
+    """Every finite bf16 as the largest of its block: the value is a finite bf16, and no code that stands for one is nearer."""
+    bits = torch.arange(0x7f80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = torch.zeros(len(bits), 32, dtype=torch.bfloat16)
+    x[:, 7] = -bits
+    codes, b = mx.quantise(x, fmt)
+    v = mx.values(mx.pack(codes, fmt), b, fmt)
+    assert torch.isfinite(v).all() and torch.equal(v.to(torch.bfloat16).double(), v)
+    grid = mx.code_values(fmt)[:len(mx.code_values(fmt)) // 2]
+    stands_for = torch.from_numpy(grid[np.isfinite(grid)])[None] * torch.exp2(b.double() - 127)      # [rows, codes]
+    stands_for[~torch.isfinite(stands_for.to(torch.bfloat16))] = float("inf")
+    best = (stands_for - bits.double()[:, None]).abs().min(-1).values
+    assert torch.equal((v[:, 7] + bits.double()).abs(), best)
