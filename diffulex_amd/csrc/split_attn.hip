@@ -467,6 +467,7 @@ struct Split {
     Seq sq;
     int kvh, row_tile;
     int lim_ctx[NB], lim_new[NB];  // this lane's rows see cached keys below lim_ctx and fresh rows below lim_new
+    int key_end, new_end;          // cached keys and fresh rows from here on are zeros in LDS (see another_pass())
     uint64_t lane_off;             // of the KV head and of this lane's chunk, in a cache row
     uint32_t my_offset;            // stage_offset()
     const int32_t* table;          // the item's block-table row
@@ -487,7 +488,7 @@ struct Split {
         const int pos = sq.key0 + t * KT + lane;
         const int p = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
         Key k;
-        k.ok = t < sq.ctx_tiles && lane < KT && pos < sq.key1 && p < a.max_pages;
+        k.ok = t < sq.ctx_tiles && lane < KT && pos < key_end && p < a.max_pages;
         k.off = pos - p * a.page_size;
         k.page = table[static_cast<uint32_t>(min(p, a.max_pages - 1))];
         return k;
@@ -579,7 +580,7 @@ struct Split {
         for (int i = 0; i < ROWS / kStep; ++i) {
             const int r = r0 + i * kStep + lane / kNewChunks, ch = lane % kNewChunks, j = t * KT + r;
             u32x4 x = {0, 0, 0, 0};
-            if (j < sq.n_new) x = *reinterpret_cast<const u32x4*>(from + (sq.new0 + static_cast<int64_t>(j)) * st + kvh * sh + ch * 8);
+            if (j < new_end) x = *reinterpret_cast<const u32x4*>(from + (sq.new0 + static_cast<int64_t>(j)) * st + kvh * sh + ch * 8);
             *reinterpret_cast<u32x4*>(to + L::chunk_offset(r, ch)) = x;
         }
     }
@@ -632,13 +633,45 @@ struct Split {
         lim_ctx[b] = ctx;
         lim_new[b] = !live ? INT32_MAX : a.block_causal ? min(sq.n_new, (t / a.dbs + 1) * a.dbs) : sq.n_new;
     }
-    DFX_D void start_item(int rows_from, bool is_group) {
+    // Returns whether its rows may see different keys of the tiles [.., u1).
+    DFX_D bool start_item(int rows_from, int u1, bool is_group, int pass) {
         lane_off = kvh * static_cast<uint64_t>(a.c_sh) + lane % kChunks * 16;
         table = a.block_tables + sq.table * a.bt_stride;
         const bool uneven = uneven_group(is_group);
         w.reset();
         start_rows(0, rows_from, uneven);
         if constexpr (NB > 1) start_rows(1, rows_from, uneven);
+        key_end = is_group && pass >= 0 ? pass : sq.key1;
+        new_end = !is_group && pass >= 0 ? pass : sq.n_new;
+        return uneven || (a.block_causal && sq.n_new > a.dbs && u1 > sq.ctx_tiles);
+    }
+    // Hidden keys that are not finite.  A hidden key's weight is 0, but 0 times an infinity or NaN is NaN: in an item whose rows do not
+    // all see the same keys (a group with contexts that end inside the prefix, blocks that do not see the later ones) it would spoil rows
+    // for which it does not exist.  Nothing in the loops looks for that; where a finished sum of such a row is NaN the item is run again for
+    // each number of keys that its rows see, `pass`, with zeros for the others and for the rows that see just these.
+    // Returns the next pass, -1: none (the same for all waves).
+    DFX_D bool spoilt(bool is_group) const {
+        bool nan = false;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) nan |= w.o[d][0][i] != w.o[d][0][i];
+        return nan && hides(is_group);
+    }
+    DFX_D bool hides(bool is_group) const { return is_group ? lim_ctx[0] < sq.key1 : lim_new[0] < sq.n_new; }
+    DFX_D bool written(bool is_group, int pass) const { return pass < 0 || (is_group ? lim_ctx[0] : lim_new[0]) == pass; }
+    DFX_D int another_pass(bool is_group, int pass, bool any_spoilt) {
+        if (pass < 0 && !__syncthreads_or(any_spoilt)) return -1;
+        const int limit = is_group ? lim_ctx[0] : lim_new[0];
+        int* least = reinterpret_cast<int*>(ml);
+        lds_barrier();
+        if (tid == 0) *least = INT32_MAX;
+        lds_barrier();
+        if (hides(is_group) && limit > pass) atomicMin(least, limit);
+        lds_barrier();
+        const int next = uniform(*least);
+        lds_barrier();
+        return next == INT32_MAX ? -1 : next;
     }
     DFX_D bool uneven_group(bool is_group) {
         if (!is_group) return false;
@@ -652,9 +685,9 @@ struct Split {
     DFX_D bool has_slot(int64_t slot) const { return slot < a.first_slot[WIDE] + a.n_slots[WIDE]; }
 
     // d block `d` of the row block from row rows_from on: a piece to its slot, or the finished rows to the output.
-    DFX_D void put(f32x16 o, int d, float inv, int rows_from, int64_t slot, bool direct) {
+    DFX_D void put(f32x16 o, int d, float inv, int rows_from, int64_t slot, bool direct, bool mine) {
         const int row = rows_from + w.col;
-        if (row >= sq.rows) return;
+        if (row >= sq.rows || !mine) return;
         if (direct) {
             const int t = row / a.group_heads, g = row - t * a.group_heads;
             uint16_t* dst = a.out + (sq.tok0 + static_cast<int64_t>(t)) * a.o_st + (static_cast<int64_t>(kvh) * a.group_heads + g) * a.o_sh;
@@ -682,9 +715,9 @@ struct Split {
     // either half: three buffers of K (scores of u + 1, u + 2, the one being written) and three of V.
     // No branch on the tile's kind in the loop and every wait for a step's loads before the next are issued: where a wait can be reached
     // with other loads in flight, the compiler waits for all of them.
-    DFX_D void wide(int u0, int u1, bool is_group, int64_t slot, bool direct) {
+    DFX_D int wide(int u0, int u1, bool is_group, int64_t slot, bool direct, int pass) {
         const int rows_from = row_tile * kWideRows + wave * 32;
-        start_item(rows_from, is_group);
+        const bool mixed = start_item(rows_from, u1, is_group, pass);
         const bool busy = rows_from < sq.rows;
         const int r0 = wave * ROWS;
         const int c1 = min(u1, sq.ctx_tiles);
@@ -780,13 +813,14 @@ struct Split {
             const float l = W::half_sum(w.l[0]);
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
-            for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, rows_from, slot + wave, direct);
-            if (!direct) ml_slot(slot + wave)[lane] = w.half ? l : w.m[0];
+            for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, rows_from, slot + wave, direct, written(is_group, pass));
+            if (!direct && written(is_group, pass)) ml_slot(slot + wave)[lane] = w.half ? l : w.m[0];
         }
+        return mixed ? another_pass(is_group, pass, spoilt(is_group)) : -1;
     }
 
     // ---- narrow --------------------------------------------------------------------------------
-    DFX_D void narrow(int u0, int u1, bool is_group, int64_t slot, bool direct) {
+    DFX_D int narrow(int u0, int u1, bool is_group, int64_t slot, bool direct, int pass) {
         uint8_t* kt = lds + wave * 2 * kMat;
         uint8_t* vt = kt + kMat;
         // wave = head of the group * side + place among the head's waves
@@ -794,7 +828,7 @@ struct Split {
         const int my_head = wave >> side_shift;
         kvh = (kvh << a.heads_shift) + my_head;
         slot += my_head;
-        start_item(row_tile * kNarrowRows, is_group);
+        const bool mixed = start_item(row_tile * kNarrowRows, u1, is_group, pass);
         int u = u0 + (wave & (side - 1));
         const int c1 = min(u1, sq.ctx_tiles);
         if (u < c1) {
@@ -848,10 +882,10 @@ struct Split {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             if (direct || has_slot(slot)) {
 #pragma unroll
-                for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, row_tile * kNarrowRows, slot, direct);
-                if (!direct) ml_slot(slot)[lane] = w.half ? l : w.m[0];
+                for (int d = 0; d < NDB; ++d) put(w.o[d][0], d, inv, row_tile * kNarrowRows, slot, direct, written(is_group, pass));
+                if (!direct && written(is_group, pass)) ml_slot(slot)[lane] = w.half ? l : w.m[0];
             }
-            return;
+            return mixed ? another_pass(is_group, pass, spoilt(is_group)) : -1;
         }
         // merge the states of a head's waves: each leaves its accumulators in its own LDS, and takes every side-th d block
         ml[wave * 64 + lane] = w.half ? l : w.m[0];
@@ -881,10 +915,11 @@ struct Split {
                     for (int j = 0; j < 4; ++j) o[4 * x + j] += f * p[j];
                 }
             }
-            if (direct || has_slot(slot)) put(o, d, inv, row_tile * kNarrowRows, slot, direct);
+            if (direct || has_slot(slot)) put(o, d, inv, row_tile * kNarrowRows, slot, direct, written(is_group, pass));
         }
-        if (!direct && (wave & (side - 1)) == 0 && has_slot(slot)) ml_slot(slot)[lane] = w.half ? sum : top;
+        if (!direct && (wave & (side - 1)) == 0 && has_slot(slot) && written(is_group, pass)) ml_slot(slot)[lane] = w.half ? sum : top;
         lds_barrier();
+        return mixed ? another_pass(is_group, pass, spoilt(is_group)) : -1;
     }
 };
 
@@ -1015,7 +1050,8 @@ __global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(con
             const int items = a.h_kv / kinds.heads * s.row_tiles, each = item_cost(kinds, s.tiles);
             if (each > 0) {
                 int j = cost < c0 ? static_cast<int>((c0 - cost) / each) : 0;
-                for (; j < items; ++j) {
+                int pass = -1;
+                for (; j < items; j += pass < 0) {
                     const int64_t from = cost + static_cast<int64_t>(j) * each;
                     if (from >= c1) break;
                     const int u0 = from >= c0 ? 0 : static_cast<int>(c0 - from);
@@ -1027,8 +1063,8 @@ __global__ void __launch_bounds__(Kind<WIDE>::kThreads, 2) split_attn_kernel(con
                     const bool is_group = v < a.n_groups;
                     const bool direct = !is_group && s.prefix == 0 && u0 == 0 && u1 == s.tiles;
                     const int64_t slot = a.first_slot[WIDE] + (static_cast<int64_t>(wg) + j) * kinds.blocks + blocks;
-                    if constexpr (WIDE) t.wide(u0, u1, is_group, slot, direct);
-                    else t.narrow(u0, u1, is_group, slot, direct);
+                    if constexpr (WIDE) pass = t.wide(u0, u1, is_group, slot, direct, pass);
+                    else pass = t.narrow(u0, u1, is_group, slot, direct, pass);
                 }
             }
             cost += static_cast<int64_t>(items) * each;

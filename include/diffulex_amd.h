@@ -529,7 +529,8 @@ int dfx_rope_kv_store(const dfx_rope_params* params, dfx_stream_t stream);
  * holds the pages of all prefix_lens[g] positions, also where its own context is shorter); every
  * sequence's keys from prefix_lens[g] on come through its own table row.  The other sequences' table entries below
  * prefix_lens[g] / page_size are not read.  A sequence whose context is shorter than its group's prefix sees its context_lens keys
- * of it.
+ * of it.  A key that a row does not see, in a prefix or among the fresh rows, never reaches it, whatever it holds; an item in which one that is
+ * not finite would have done so is computed again, once for each number of keys that its rows see.
  *
  * Two or three launches (pieces of many rows, pieces of few, merge), planned on the device from the lengths: nothing is read back, they
  * may be recorded into a graph whose replays find other lengths, and the results do not depend on timing (pieces are merged in order).  The workspace

@@ -493,3 +493,57 @@ def test_two_calls_at_once_on_two_streams(dev):
     for ga, gb in got:
         a.check(ga.cpu(), wa)
         b.check(gb.cpu(), wb)
+
+
+def _check_with_non_finite(p, got, want):
+    """NaN and infinities where the oracle has them, its values within the tolerance elsewhere."""
+    o, spread, written = want
+    assert (got[~written] == 77.0).all()
+    got = got.double()
+    assert torch.equal(torch.isnan(got)[written], torch.isnan(o)[written])
+    inf = torch.isinf(o) & written[:, None, None]
+    assert (got[inf] == o[inf]).all()
+    ok = torch.isfinite(o) & written[:, None, None]
+    tol = 2.0 ** -8 * (1 + 1 / 16) * (spread + o.abs()) + 1e-7
+    assert ((got - o).abs() <= tol)[ok].all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("new", [1, 9])
+@pytest.mark.parametrize("hq,hkv,hd", [(28, 4, 128), (4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("n_wg", [0, 3, 40])
+def test_non_finite_values_of_a_prefix_reach_the_rows_that_see_them_only(dev, fmt, new, hq, hkv, hd, n_wg):
+    """Values of two keys of a shared prefix are infinite or NaN; some sequences of the group end before the second, or before
+    both, one has no context at all: for them these keys do not exist, whatever shares their tiles."""
+    p = Problem(fmt, [200, 40, 230, 0, 130, 200, 90], [new] * 7, hq, hkv, hd, 16, seed=70, groups=[(0, 7, 200)])
+    for pos in (70, 150):
+        at, off = int(p.table[0, pos // 16]), pos % 16
+        if fmt == "bf16":
+            p.vc[at, off, 0, 3], p.vc[at, off, -1, 40], p.vc[at, off, -1, 41] = float("nan"), float("inf"), float("-inf")
+        else:
+            p.vs[at, off, 0, 0] = p.vs[at, off, -1, 1] = 255
+    p.vv = p.vc.double() if fmt == "bf16" else mx.values(p.vc, p.vs, fmt)
+    want = p.want()
+    rows = torch.arange(7).repeat_interleave(new)
+    clean = (rows == 1) | (rows == 3)
+    assert torch.isfinite(want[0][clean]).all() and not torch.isfinite(want[0][~clean]).flatten(1).all(-1).any()
+    _check_with_non_finite(p, p.run(dev, max_workgroups=n_wg), want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hq,hkv,hd", [(28, 4, 128), (4, 2, 64), (1, 1, 128)])
+@pytest.mark.parametrize("n_wg", [0, 5])
+def test_non_finite_values_of_fresh_rows_reach_the_blocks_that_see_them_only(dev, fmt, hq, hkv, hd, n_wg):
+    p = Problem(fmt, [50, 0, 300], [12, 9, 40], hq, hkv, hd, 16, seed=71, block_causal=True, dbs=4)
+    bad = {0: 6, 1: 8, 2: 37}                              # sequence: fresh row, in its blocks 1, 2 and 9
+    clean = Problem(fmt, [50, 0, 300], [12, 9, 40], hq, hkv, hd, 16, seed=71, block_causal=True, dbs=4)
+    sees = torch.zeros(p.q.shape[0], dtype=torch.bool)
+    for s, j in bad.items():
+        a = int(p.cu[s])
+        p.v[a + j, :, 5], p.v[a + j, :, 33] = float("nan"), float("inf")
+        sees[a + j // 4 * 4:int(p.cu[s + 1])] = True
+    got = p.run(dev, max_workgroups=n_wg)
+    assert torch.isnan(got[sees][..., 5]).all() and (got[sees][..., 33] == float("inf")).all()
+    want = clean.want()
+    keep = ~sees[:, None, None].expand_as(got) | (torch.arange(hd) != 5) & (torch.arange(hd) != 33)
+    clean.check(torch.where(keep, got.double(), want[0]), want)
