@@ -542,6 +542,11 @@ void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& k
                 "cos_sin_cache: contiguous fp32 device tensor");
     int64_t hq, hk;
     const int64_t tq = rows_of(query, head_size, hq, "query"), tk = rows_of(key, head_size, hk, "key");
+    int64_t hqo, hko;
+    TORCH_CHECK(rows_of(q_out, head_size, hqo, "q_out") == tq && rows_of(k_out, head_size, hko, "k_out") == tk && hqo == hq && hko == hk,
+                "q_out and k_out have the rows and heads of query and key");
+    auto here = [&](const Tensor& t) { TORCH_CHECK(t.device() == query.device(), "all tensors on one device"); };
+    for (const Tensor* t : {&positions, &key, static_cast<const Tensor*>(&q_out), static_cast<const Tensor*>(&k_out), &cos_sin_cache}) here(*t);
     TORCH_CHECK(positions.is_contiguous() && tq == tk && tq == positions.numel(), "one position per token row of query and key");
     dfx_rope_params p = {};
     p.q = query.data_ptr();
@@ -569,6 +574,9 @@ void rope_kv_store(const Tensor& positions, const Tensor& query, const Tensor& k
         const int64_t tv = rows_of(*value, head_size, hv, "value");
         const int64_t row = hk * head_size;
         TORCH_CHECK(tv == tk && hv == hk, "value does not fit key");
+        for (const OptTensor* t : {&value, static_cast<const OptTensor*>(&k_cache), static_cast<const OptTensor*>(&v_cache), &slot_mapping,
+                                   static_cast<const OptTensor*>(&k_scale), static_cast<const OptTensor*>(&v_scale)})
+            if (has(*t)) here(**t);
         const bool distinct = k_cache->dim() == 5;   // K [pages, H_kv, hd / 8, page, 8], V [pages, H_kv, hd, page]
         if (distinct) {
             TORCH_CHECK(v_cache->dim() == 4 && k_cache->size(1) == hk && v_cache->size(1) == hk && k_cache->size(4) == 8 &&

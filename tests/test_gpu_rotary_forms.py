@@ -163,3 +163,28 @@ def test_refusals(dev):
         rope(pos[:3], x, x)
     with pytest.raises(RuntimeError):
         rope(pos, x.half(), x)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tensors_the_kernel_cannot_reach_are_refused(dev, interleaved):
+    """Positions, slots, caches or scales in host memory, outputs of other shapes: an error before anything is launched."""
+    op = _lib.ops().rope_kv_store
+    t, hq, hk, hd = 4, 4, 2, 64
+    bf = dict(dtype=torch.bfloat16, device=dev)
+    q, k, v = torch.zeros(t, hq * hd, **bf), torch.zeros(t, hk * hd, **bf), torch.zeros(t, hk * hd, **bf)
+    good = dict(positions=torch.arange(t, device=dev), query=q, key=k, q_out=torch.empty_like(q), k_out=torch.empty_like(k),
+                cos_sin_cache=torch.zeros(8, hd, device=dev), head_size=hd, value=v,
+                k_cache=torch.zeros(2, 16, hk, hd, dtype=torch.uint8, device=dev), v_cache=torch.zeros(2, 16, hk, hd, dtype=torch.uint8, device=dev),
+                slot_mapping=torch.arange(t, device=dev), k_scale=torch.zeros(2, 16, hk, hd // 32, dtype=torch.uint8, device=dev),
+                v_scale=torch.zeros(2, 16, hk, hd // 32, dtype=torch.uint8, device=dev), rotary_dim=0, interleaved=interleaved)
+    fp8 = dict(good, k_scale=torch.ones(hk, device=dev), v_scale=torch.ones(hk, device=dev))
+    for args in (good, fp8):
+        op(**args)
+        for name in ("positions", "cos_sin_cache", "value", "k_cache", "v_cache", "slot_mapping", "k_scale", "v_scale", "q_out", "k_out"):
+            with pytest.raises(RuntimeError):
+                op(**dict(args, **{name: args[name].cpu()}))
+        for bad in (dict(q_out=torch.empty(t - 1, hq * hd, **bf)), dict(k_out=torch.empty(t, hd, **bf)), dict(q_out=torch.empty(t, hq * hd, device=dev)),
+                    dict(k_out=torch.empty(t, 2 * hk * hd, **bf)[:, ::2])):
+            with pytest.raises(RuntimeError):
+                op(**dict(args, **bad))
+    torch.cuda.synchronize()
