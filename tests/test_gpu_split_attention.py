@@ -547,3 +547,21 @@ def test_non_finite_values_of_fresh_rows_reach_the_blocks_that_see_them_only(dev
     want = clean.want()
     keep = ~sees[:, None, None].expand_as(got) | (torch.arange(hd) != 5) & (torch.arange(hd) != 33)
     clean.check(torch.where(keep, got.double(), want[0]), want)
+
+
+@pytest.mark.parametrize("n_wg", [0, 1, 30])
+@pytest.mark.parametrize("new", [1, 40])
+def test_an_infinite_key(dev, new, n_wg):
+    """An element of one cached key is infinite: its score is +inf for the rows whose element there is positive -- they have no softmax, NaN --
+    and -inf for the others, which go on as if the key were not there."""
+    p = Problem("bf16", [300, 64], [new, new], 8, 2, 128, 16, seed=72)
+    p.q[:, :, 9] = torch.where(p.q[:, :, 9] == 0, torch.ones_like(p.q[:, :, 9]), p.q[:, :, 9])
+    p.kc[int(p.table[0, 7]), 3, :, 9] = float("inf")
+    p.kv = p.kc.double()
+    nan = (p.q[:, :, 9] > 0) & (torch.arange(2 * new) < new)[:, None]
+    assert nan.any() and not nan[:new].all()
+    got = p.run(dev, max_workgroups=n_wg)
+    assert torch.isnan(got[nan]).all() and not torch.isnan(got[~nan]).any()
+    p.kv[int(p.table[0, 7]), 3, :, 9] = 1e9                # for the oracle: weight exp(-1e9 |q|) = 0 in 64 bits where the element is negative
+    o, spread, written = p.want()
+    p.check(torch.where(nan[..., None], o, got.double()), (o, spread, written))
