@@ -3,7 +3,7 @@
 // Both are bound by memory.  Store: one lane per 8 elements of a K row and of a V row (16-byte loads); a block of 32 elements
 // is four neighbouring lanes, which agree on its largest magnitude in two lane permutations, so that codes and scales
 // are written in the same pass that reads the rows.  Load: one lane per 8 elements as well, 16-byte stores of bf16.
-// Measured: 16385 rows of 32 heads of 128 stored as E4M3 in 77 us (5.3 TB/s, what a large copy reaches); 256 rows of 4 heads in 7.2 us (the
+// Measured: 16385 rows of 32 heads of 128 stored as E4M3 in 76 us (5.3 TB/s, what a large copy reaches); 256 rows of 4 heads in 7.1 us (the
 // launch); 64 sequences of 256 to 2048 E4M3 rows of 4 heads loaded in 62 us
 // (4.2 TB/s; 42 us when the same tensors are loaded again).  The load writes twice what it reads, or more, and past L2: written through it, the same
 // took 66 us (65 again), and 3 sequences of 9000 to 33000 E2M1 rows with the store of 5 before them 37 us instead of 23.  More chunks in flight per

@@ -252,10 +252,11 @@ int launch_rope_distinct(const RopeArgs& a, const void* positions, const void* s
 //
 // A work item is 16 elements of a head row and 32 bytes of it: both chunks of a pair of halves, 16 neighbouring elements
 // otherwise, so that whoever reads an element is the one who writes it (in place is safe).  The rows are moved once
-// and the angles come from L1 (every head of a token reads the same table row), so memory bounds it.  kUnroll items per
-// thread are loaded before the first is used: one item's loads in flight per thread left the launch waiting on latency.
+// and the angles come from L1 (every head of a token reads the same table row), so memory bounds it where there are many tokens.  kUnroll
+// items per thread are read before the first is rotated; as compiled, the branch on the positions' type ends each item's reads with a wait for all
+// loads, and its angles and slot are read in the second loop: up to twelve trips to memory one after the other, which a small launch waits for.
 // Measured: 65521 tokens of 28 + 4 heads of 128 with 64 elements rotated in 209 us (5.2 TB/s, what a large copy reaches); 2048 tokens with the
-// store into an E4M3 cache in 14 us; 64 tokens in 12 us, of which the launch's host side is the larger part.
+// store into an E4M3 cache in 14 us (the kernel 11 to 12); 64 tokens in 12 us, the kernel 4.6, the rest the call's host side.
 constexpr int kUnroll = 4;
 constexpr int kStoreNone = 0, kStoreBf16 = 1, kStoreFp8 = 2, kStoreMx8 = 3, kStoreMx4 = 4;
 

@@ -17,14 +17,17 @@
 //   narrow (single tokens, small blocks): bound by memory.  32 rows; four waves, each with a KV head of its own where there are
 //     four (a token's codes and scales of neighbouring heads lie in the same memory lines: the waves of a workgroup should want them
 //     at the same time), with every second or fourth tile of a head otherwise, whose softmax states are then merged in LDS.
-//     A wave moves its 32-key tiles into LDS of its own: no barrier in the loop, the next tiles' loads in flight over the arithmetic.
-//     5 single tokens of 32 / 32 heads over 20000 to 60000 E2M1 keys: 274 us, 3.0 TB/s (425 us with a workgroup's waves on four tiles of one
+//     A wave moves its 32-key tiles into LDS of its own: no barrier in the loop, the next tiles' loads issued before the arithmetic
+//     (how far they stay in flight over it: kDepth).
+//     5 single tokens of 32 / 32 heads over 20000 to 60000 E2M1 keys: 275 us, 3.0 TB/s (425 us with a workgroup's waves on four tiles of one
 //     head: a head's 4 scale bytes and 64 codes are a part of a memory line each).
 //   wide: bound by the matrix instructions and the exponentials.  256 rows, 32 for each of eight waves, over 64-key tiles shared by the
 //     waves; in each wave the products of one tile's scores run beside the exponentials of the tile before.
 //     128 sequences of 32 tokens, 28 / 4 heads, over 2048 to 8192 E4M3 keys: 420 to 455 us, 680 to 735 TFLOP/s of the rows' own products (224 of a tile's
 //     256 rows).  Two row blocks per wave (half the LDS reads) do not fit the registers; one launch for both kinds, sharing the workgroups out,
 //     gained 7 us where a prefix of 4096 serves 64 single tokens and lost 8 to 17 us elsewhere.
+// At head_dim 128 both kinds take all 256 registers and spill some 60 to 85: the wide ones around an item (bf16 four in a tile's step as well), the
+// narrow ones in the loop.
 // Microscaled codes are widened on the way from registers to LDS, once per tile, with their block's scale applied by the same
 // instruction: from there on the arithmetic is the bf16 cache's.
 #include "attn_tile.h"
@@ -37,7 +40,8 @@ constexpr int kNarrowRows = 32, kWideRows = 256;
 constexpr int kNarrowKeys = 32, kWideKeys = 64;
 // Rows of a virtual sequence up to which its items are narrow.  Each tile of 32 rows reads the keys again, a wide tile costs the same whatever its rows.
 // (Narrow against wide, E4M3, 4 KV heads, us: 32 rows over 4096 keys, 64 sequences: 110, 123; 64 rows: 143, 137; 96 rows: 219, 141, a bf16 cache 356,
-// 176; 96 rows, 4 sequences: 47, 38; 64 rows over 700 keys, 128 sequences: 79, 87; 84 rows over 16 to 700 keys beside 4 prefixes of 8192: 320, 337.)
+// 176; 96 rows, 4 sequences: 47, 38; 64 rows over 700 keys, 128 sequences: 79, 87; 84 rows over 16 to 700 keys beside 4 prefixes of 8192: 320, 337:
+// by the rows alone the last two take the slower side, by 5 to 10 %, for the 4 to 50 % of the others.)
 constexpr int kNarrowMost = 32;
 // Beside its units (cost 1 each) an item costs its start and end: queries, first tiles, the merge of the waves, the rows written.
 // (Narrow: of the tiles that the waves of a head take side by side; a unit is one such tile.)
@@ -323,8 +327,8 @@ struct Wave {
     }
 
     DFX_D float base_of(int b) const { return m[b] == -INFINITY ? 0.0f : m[b]; }
-    // Weights of 16 keys (score registers 8 x .. 8 x + 7), rounded to bf16 for the second product; returns the sum of the
-    // unrounded ones.
+    // Weights of 16 keys (score registers 8 x .. 8 x + 7), rounded to bf16 for the second product (its matrix instruction takes two bf16 operands,
+    // and V has no more; half a step, 2^-8 of a weight, as the rounded output's own); returns the sum of the unrounded ones.
     static DFX_D float weights8(const f32x16& s, int x, float c, float base, bf16x8& p) {
         float e[8];
 #pragma unroll
@@ -453,8 +457,9 @@ struct Split {
     static constexpr int kAccBytes = 32 * HD * 4;
     static constexpr int kPer = 64 / kChunks;                                          // rows per load of the wave
     static constexpr int kLoads = ROWS > kPer ? ROWS / kPer : 1;                       // (one that some lanes only repeat, where ROWS < kPer)
-    // Tiles in flight per wave of a narrow item.  The eight waves of a compute unit should have some 100 KB on the way; a bf16
-    // tile is 16 KB.
+    // Tiles in flight per wave of a narrow item, as far as the source goes: the eight waves of a compute unit should have some 100 KB on the way; a
+    // bf16 tile is 16 KB.  Compiled for head_dim 128, E4M3 reloads spilled registers right behind a tile's loads, which waits for them all (no tile
+    // stays in flight over the arithmetic), E2M1 waits for all loads in the first of its three steps only, bf16 reloads in front of its loads.
     static constexpr int kDepth = KV == kBf16 ? 1 : KV == kMx8 ? 2 : 3;
     static constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << 32) - 1;
 
@@ -573,7 +578,7 @@ struct Split {
             }
         }
     }
-    // Fresh rows (bf16 operands) of fresh tile t: straight to LDS, there are few of them.
+    // Fresh rows (bf16 operands) of fresh tile t: straight to LDS, one after the other (a branch and a wait each), there are few of them.
     DFX_D void fresh_rows(const uint16_t* from, int64_t st, int64_t sh, int t, uint8_t* to, int r0) const {
         constexpr int kStep = 64 / kNewChunks;
 #pragma unroll
@@ -835,7 +840,8 @@ struct Split {
             Stage sk[kDepth], sv[kDepth];
             uint64_t valid[kDepth];
             // A table entry is looked up kDepth tiles before its rows' loads are issued, so that it is in front of the loads that a tile's
-            // commit waits for: loads return in order, and a wait for a younger entry would drain the tiles in flight.
+            // commit waits for: loads return in order, and a wait for a younger entry would drain the tiles in flight (as reloads of spilled
+            // registers do: see kDepth).
             Key keys[kDepth];
 #pragma unroll
             for (int i = 0; i < kDepth; ++i) keys[i] = look_up(u + i * side);
